@@ -443,6 +443,128 @@ class Model:
             pass
 
 
+# ---------------------------------------------------------------- serving operators (gmoe_serve.h)
+_BATCH_SIZES = ["n_requests", "max_tokens", "max_pages", "page_size"]
+_BATCH_ARRAYS = ["seen", "fresh", "free_pages", "n_free", "table", "offsets", "context", "request", "position", "slot",
+                 "totals"]
+
+
+class GmoeBatch(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in _BATCH_SIZES] + [(n, C.c_void_p) for n in _BATCH_ARRAYS]
+
+
+class GmoeKv4(C.Structure):
+    _fields_ = [("rows", C.c_void_p), ("kv_lora_rank", C.c_int32), ("rope_dim", C.c_int32), ("n_pages", C.c_int32),
+                ("page_size", C.c_int32)]
+
+
+class GmoeKv4Heads(C.Structure):
+    _fields_ = [("n_heads", C.c_int32), ("scale", C.c_float), ("q_abs", C.c_void_p), ("ld_q_abs", C.c_int64),
+                ("q_pe", C.c_void_p), ("ld_q_pe", C.c_int64), ("out", C.c_void_p), ("ld_out", C.c_int64),
+                ("work", C.c_void_p), ("work_bytes", C.c_size_t)]
+
+
+class GmoeLogprobsArgs(C.Structure):
+    _fields_ = [("n", C.c_int32), ("vocab", C.c_int32), ("n_given", C.c_int32), ("top", C.c_int32),
+                ("logits", C.c_void_p), ("ld", C.c_int64), ("given", C.c_void_p), ("logprob", C.c_void_p),
+                ("entropy", C.c_void_p), ("top_id", C.c_void_p), ("top_logprob", C.c_void_p), ("work", C.c_void_p),
+                ("work_bytes", C.c_size_t)]
+
+
+def serve_lib():
+    lib = gmoe_lib()
+    if not getattr(lib, "_serve_typed", False):
+        P, I, L = C.c_void_p, C.c_int, C.c_int64
+        lib.gmoe_page_maps.argtypes = [I, P, P]
+        lib.gmoe_kv4_row_bytes.argtypes = [I, I]
+        lib.gmoe_kv4_append.argtypes = [I, P, I, P, L, P, L, P, P]
+        lib.gmoe_kv4_read.argtypes = [I, P, I, P, P, L, P, L, P]
+        lib.gmoe_kv4_attend.argtypes = [I, P, P, P, P]
+        lib.gmoe_kv4_attend_workspace.argtypes = [I, I]
+        lib.gmoe_logprobs.argtypes = [I, P, P]
+        lib.gmoe_logprobs_workspace.argtypes = [I, I, I]
+        for f in ("gmoe_page_maps", "gmoe_kv4_append", "gmoe_kv4_read", "gmoe_kv4_attend", "gmoe_logprobs"):
+            getattr(lib, f).restype = C.c_int
+        for f in ("gmoe_kv4_row_bytes", "gmoe_kv4_attend_workspace", "gmoe_logprobs_workspace"):
+            getattr(lib, f).restype = C.c_size_t
+        lib._serve_typed = True
+    return lib
+
+
+class Batch:
+    """The requests of a step (gmoe_batch) over the caller's device arrays, given by address; maps()
+    fills table, offsets, context, request, position, slot and totals."""
+
+    def __init__(self, n_requests, max_tokens, max_pages, page_size, device=0, free=None, **arrays):
+        if free is not None:
+            arrays["free_pages"] = free
+        self.lib, self.device = serve_lib(), device
+        self.c = GmoeBatch(n_requests, max_tokens, max_pages, page_size, *[arrays.pop(n, None) for n in _BATCH_ARRAYS])
+        if arrays:
+            raise TypeError(f"no such arrays: {sorted(arrays)}")
+        self.ref = C.addressof(self.c)
+
+    def maps(self, stream=None):
+        rc = self.lib.gmoe_page_maps(self.device, self.ref, stream)
+        if rc:
+            check(rc, "gmoe_page_maps")
+
+
+class Cache4:
+    """One layer's paged latent cache in 4 bits (gmoe_kv4) over the caller's device memory at `rows`:
+    n_pages * page_size rows of row_bytes(kv, rope)."""
+
+    def __init__(self, rows, kv_lora_rank, rope_dim, n_pages, page_size, device=0):
+        self.lib, self.device = serve_lib(), device
+        self.c = GmoeKv4(rows, kv_lora_rank, rope_dim, n_pages, page_size)
+        self.heads = GmoeKv4Heads()
+        self.ref, self.href = C.addressof(self.c), C.addressof(self.heads)
+
+    @staticmethod
+    def row_bytes(kv_lora_rank, rope_dim):
+        return int(serve_lib().gmoe_kv4_row_bytes(kv_lora_rank, rope_dim))
+
+    def append(self, n, comp, ld_comp, pe, ld_pe, slot, stream=None):
+        rc = self.lib.gmoe_kv4_append(self.device, self.ref, n, comp, ld_comp, pe, ld_pe, slot, stream)
+        if rc:
+            check(rc, "gmoe_kv4_append")
+
+    def read(self, n, slot, comp, ld_comp, pe, ld_pe, stream=None):
+        rc = self.lib.gmoe_kv4_read(self.device, self.ref, n, slot, comp, ld_comp, pe, ld_pe, stream)
+        if rc:
+            check(rc, "gmoe_kv4_read")
+
+    def attend_workspace(self, n_heads):
+        return int(self.lib.gmoe_kv4_attend_workspace(n_heads, self.c.kv_lora_rank))
+
+    def attend(self, batch, n_heads, scale, q_abs, ld_q_abs, q_pe, ld_q_pe, out, ld_out, work, work_bytes, stream=None):
+        h = self.heads
+        h.n_heads, h.scale, h.q_abs, h.ld_q_abs, h.q_pe, h.ld_q_pe = n_heads, scale, q_abs, ld_q_abs, q_pe, ld_q_pe
+        h.out, h.ld_out, h.work, h.work_bytes = out, ld_out, work, work_bytes
+        rc = self.lib.gmoe_kv4_attend(self.device, self.ref, batch.ref, self.href, stream)
+        if rc:
+            check(rc, "gmoe_kv4_attend")
+
+
+class LogProbs:
+    """gmoe_logprobs for calls of one size: n rows over vocab tokens, n_given given tokens and top
+    alternatives a row; `workspace` is the bytes of its workspace."""
+
+    def __init__(self, n, vocab, top, n_given, device=0):
+        self.lib, self.device = serve_lib(), device
+        self.c = GmoeLogprobsArgs(n, vocab, n_given, top)
+        self.ref = C.addressof(self.c)
+        self.workspace = int(self.lib.gmoe_logprobs_workspace(n, vocab, top))
+
+    def __call__(self, logits, ld, given, logprob, entropy, top_id, top_logprob, work, work_bytes, stream=None):
+        a = self.c
+        a.logits, a.ld, a.given, a.logprob, a.entropy = logits, ld, given, logprob, entropy
+        a.top_id, a.top_logprob, a.work, a.work_bytes = top_id, top_logprob, work, work_bytes
+        rc = self.lib.gmoe_logprobs(self.device, self.ref, stream)
+        if rc:
+            check(rc, "gmoe_logprobs")
+
+
 # ---------------------------------------------------------------- HIP runtime (ctypes)
 _hip = None
 HIP_H2D, HIP_D2H, HIP_D2D = 1, 2, 3
