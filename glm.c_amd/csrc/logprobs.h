@@ -1,23 +1,54 @@
 // logprobs.h -- log probabilities of given tokens, entropy and top alternatives of rows of logits
-// (gmoe_logprobs).
+// (gmoe_logprobs), in one pass over the logits.
 //
-// With m a row's largest logit and S the sum of exp(x - m) over every other token, ln p = (x - m) -
-// log1p(S) and the entropy is log1p(S) + sum p (m - x): sums of terms of one sign, which keep their
-// relative precision where one token has nearly all of p (S far below 1).
+// Mathematics. With m a row's largest logit and S the sum of exp(x - m) over every other token,
+// ln p = (x - m) - log1p(S) and the entropy is log1p(S) + D / (1 + S), D = sum exp(x - m) (m - x): sums
+// of terms of one sign, which keep their relative precision where one token has nearly all of p
+// (S far below 1). (m, S, D) of two parts join by moving the part of the lower m to the higher:
+// S' = f S, D' = f (D + dm S), f = e^-dm, and the lower m itself joins as one more term. A thread
+// keeps a triple of its own, so the pass has no exchange; a tile's values meet in a knockout
+// (max and min of pairs), whose winner is the tile's maximum and whose losers are the terms.
+//
+// Top alternatives. Keys order the logits by value, then the lower index, and no two are
+// equal. A block keeps the list of keys that may be among its `top` largest: those above a
+// threshold, which starts as the top-th largest of the first tile's per-thread maxima (at least
+// `top` values are no smaller) and is set to the list's top-th key each time the list is cut
+// to `top`. After the first tiles nearly no value passes, so that a tile costs one comparison a
+// thread. Later tiles hold higher indexes, so a value equal to the threshold does not pass.
+//
+// Split. A block takes a run of tiles of a row; with more than one run a row (few rows) the
+// runs' triples and keys go through the workspace and k_lp_join joins them, a block a row.
 #pragma once
+
+#include <float.h>
 
 #include "common.h"
 #include "gmoe_serve.h"
+#include "pages.h"
 
 #define LP_BLOCK 256
+#define LP_SEGS 256     // most runs of a row: a thread each in k_lp_join
+#define LP_LIST 512     // list entries besides a tile's
+#define LP_CUT 160      // the list is cut to `top` when it is longer
+
+// A run's result: the triple, its keys' number, whether a value is NaN.
+struct LpRun {
+    float m, s, d;
+    int n;  // -1: a NaN
+};
+
+struct LpArgs {
+    gmoe_logprobs_args a;
+    int segs, per;  // runs a row, tiles a run
+    LpRun *runs;                // [n][segs]
+    unsigned long long *keys;   // [n][segs][top], the largest first
+};
 
 // A value and its index as one integer that orders rows of logits: by value, then the lower index
-// first; a NaN above every number. 0 is below every key.
+// first. Not for NaN. 0 is below every key.
 __device__ static inline unsigned long long lp_key(float x, int i) {
-    const unsigned b = __float_as_uint(x);
-    unsigned o = b & 0x80000000u ? ~b : b | 0x80000000u;
-    if (x != x) o = 0xffffffffu;
-    if (b == 0x80000000u) o = 0x80000000u;  // -0 equals +0
+    const unsigned b = __float_as_uint(x + 0.0f);  // (-0 equals +0)
+    const unsigned o = b & 0x80000000u ? ~b : b | 0x80000000u;
     return (unsigned long long)o << 32 | (unsigned)~i;
 }
 __device__ static inline float lp_value(unsigned long long key) {
@@ -26,69 +57,311 @@ __device__ static inline float lp_value(unsigned long long key) {
 }
 __device__ static inline int lp_index(unsigned long long key) { return (int)~(unsigned)key; }
 
-__device__ static inline unsigned long long wave_max_u64(unsigned long long v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        const unsigned long long o = __shfl_xor(v, d);
-        v = o > v ? o : v;
-    }
-    return v;
-}
+// e^y for y <= 0 (0 for -inf): the product's rounding is 2^-24 |y| of a result of e^y.
+__device__ static inline float lp_exp(float y) { return __builtin_amdgcn_exp2f(y * 1.44269504f); }
 
-// A plain form: a block a row, one pass for each alternative.
-__global__ __launch_bounds__(LP_BLOCK) void k_logprobs(gmoe_logprobs_args a) {
-    __shared__ unsigned long long rk[LP_BLOCK / 64];
-    __shared__ float rs[2][LP_BLOCK / 64];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, V = a.vocab;
-    const float *x = a.logits + blockIdx.x * a.ld;
-    auto below = [&](unsigned long long lim) {  // the row's largest key under lim
-        unsigned long long best = 0;
-        for (int i = tid; i < V; i += LP_BLOCK) {
-            const unsigned long long k = lp_key(x[i], i);
-            if (k < lim && k > best) best = k;
-        }
-        best = wave_max_u64(best);
-        __syncthreads();
-        if (lane == 0) rk[w] = best;
-        __syncthreads();
-        for (int k = 0; k < LP_BLOCK / 64; k++) best = rk[k] > best ? rk[k] : best;
-        return best;
-    };
-    const unsigned long long top = below(~0ull);
-    const float m = lp_value(top);
-    const int im = lp_index(top);
-    const bool none = m == -INFINITY, bad = !(m < INFINITY);
-    float s = 0.0f, d = 0.0f;
-    for (int i = tid; i < V; i += LP_BLOCK) {
-        const float y = x[i] - m, e = expf(y);
-        if (i != im) s += e;
-        if (e > 0.0f) d = fmaf(e, -y, d);
+struct LpSum {
+    float m, s, d;
+    // The running sums moved to a reference of at least m.
+    __device__ inline void move(float ref) {
+        const float f = lp_exp(m - ref), dm = fminf(ref - m, 1000.0f);  // (f is 0 by then)
+        d = f * fmaf(dm, s, d);
+        s *= f;
     }
+    __device__ inline void term(float x, float ref) {
+        const float y = x - ref, e = lp_exp(y);
+        s += e;
+        d = fmaf(-e, fmaxf(y, -1000.0f), d);  // (0 * inf is no term)
+    }
+};
+
+// The block's triples joined into one, in every thread; red: 3 * LP_BLOCK / 64 floats.
+__device__ static inline LpSum lp_join(LpSum v, float *red) {
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    constexpr int W = LP_BLOCK / 64;
+    float M = v.m;
+#pragma unroll
+    for (int k = 32; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor(M, k));
+    __syncthreads();
+    if (lane == 0) red[w] = M;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < W; k++) M = fmaxf(M, red[k]);
+    int first = 0;  // the first wave that holds the maximum: its first such lane's own term is left out
+    while (first < W - 1 && red[first] != M) first++;
+    const unsigned long long has = __ballot(v.m == M);
+    const bool mine = w == first && has && lane == __ffsll((unsigned long long)has) - 1;
+    const float ref = fmaxf(M, -FLT_MAX), m0 = v.m;
+    v.move(ref);
+    if (!mine) v.term(m0, ref);
+#pragma unroll
     for (int k = 32; k > 0; k >>= 1) {
-        s += __shfl_xor(s, k);
-        d += __shfl_xor(d, k);
+        v.s += __shfl_xor(v.s, k);
+        v.d += __shfl_xor(v.d, k);
     }
     if (lane == 0) {
-        rs[0][w] = s;
-        rs[1][w] = d;
+        red[W + w] = v.s;
+        red[2 * W + w] = v.d;
     }
     __syncthreads();
-    s = (rs[0][0] + rs[0][1]) + (rs[0][2] + rs[0][3]);
-    d = (rs[1][0] + rs[1][1]) + (rs[1][2] + rs[1][3]);
-    const float nan = __uint_as_float(0x7fc00000u), ls = log1pf(s);
-    auto lp = [&](float v) { return bad ? nan : none ? -INFINITY : (v - m) - ls; };
-    if (tid == 0 && a.entropy) a.entropy[blockIdx.x] = bad ? nan : none ? 0.0f : ls + d / (1.0f + s);
-    for (int g = tid; g < a.n_given; g += LP_BLOCK) {
-        const int id = a.given[(size_t)blockIdx.x * a.n_given + g];
-        a.logprob[(size_t)blockIdx.x * a.n_given + g] = id < 0 || id >= V ? nan : lp(x[id]);
+    v.m = M;
+    v.s = (red[W] + red[W + 1]) + (red[W + 2] + red[W + 3]);
+    v.d = (red[2 * W] + red[2 * W + 1]) + (red[2 * W + 2] + red[2 * W + 3]);
+    return v;
+}
+static_assert(LP_BLOCK == 256, "lp_join adds four waves");
+
+// The list of keys of a block, in shared memory, with what cutting it needs.
+template <int CAP>
+struct LpList {
+    unsigned long long key[CAP];
+    unsigned long long best[GMOE_TOP_MAX];
+    unsigned hist[256];
+    unsigned scan[LP_BLOCK / 64];
+    unsigned n, digit, left, fill;
+};
+
+// Cuts the list's first n keys to its `top` largest (n where there are fewer), the largest first,
+// and returns how many those are; every thread calls it with the same n, after a barrier.
+template <int CAP>
+__device__ static int lp_cut(LpList<CAP> &l, int n, int top) {
+    const int tid = threadIdx.x;
+    const unsigned long long *src = l.key;
+    if (n > 2 * LP_BLOCK) {
+        // the top-th largest key, digit by digit from the highest: `left` of the keys that
+        // share the digits so far are wanted
+        unsigned long long prefix = 0;
+        int shift = 56;
+        unsigned left = top;
+        for (;; shift -= 8) {
+            l.hist[tid] = 0;
+            __syncthreads();
+            for (int i = tid; i < n; i += LP_BLOCK) {
+                const unsigned long long k = l.key[i];
+                if (shift == 56 || k >> (shift + 8) == prefix) atomicAdd(&l.hist[(k >> shift) & 255], 1u);
+            }
+            __syncthreads();
+            const unsigned c = l.hist[255 - tid];
+            unsigned all;
+            const unsigned above = block_scan_u(c, l.scan, &all);
+            if (above < left && left <= above + c) {
+                l.digit = 255 - tid;
+                l.left = left - above;
+                l.fill = c;
+            }
+            __syncthreads();
+            prefix = prefix << 8 | l.digit;
+            left = l.left;
+            const bool whole = left == l.fill;  // the whole bin is wanted
+            __syncthreads();
+            if (whole || shift == 0) break;
+        }
+        const unsigned long long least = prefix << shift;
+        if (tid == 0) l.fill = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += LP_BLOCK)
+            if (l.key[i] >= least) l.best[atomicAdd(&l.fill, 1u)] = l.key[i];
+        __syncthreads();
+        src = l.best;
+        n = top;
     }
-    unsigned long long lim = ~0ull;
-    for (int k = 0; k < a.top; k++) {
-        lim = below(lim);
-        if (tid == 0) {
-            const bool no = lim == 0;
-            a.top_id[(size_t)blockIdx.x * a.top + k] = no || bad || none ? -1 : lp_index(lim);
-            a.top_logprob[(size_t)blockIdx.x * a.top + k] = bad ? nan : no ? -INFINITY : lp(lp_value(lim));
+    // ranked by counting the larger ones
+    const unsigned long long k0 = tid < n ? src[tid] : 0, k1 = tid + LP_BLOCK < n ? src[tid + LP_BLOCK] : 0;
+    int r0 = 0, r1 = 0;
+    for (int j = 0; j < n; j++) {
+        const unsigned long long k = src[j];
+        r0 += k > k0;
+        r1 += k > k1;
+    }
+    __syncthreads();
+    if (tid < n && r0 < top) l.key[r0] = k0;
+    if (tid + LP_BLOCK < n && r1 < top) l.key[r1] = k1;
+    __syncthreads();
+    return min(n, top);
+}
+
+// The row's results from its joined triple and its alternatives (k of them, the largest first).
+__device__ static inline void lp_finish(const gmoe_logprobs_args &a, int row, const LpSum &t, bool nan, const unsigned long long *key,
+                                        int k) {
+    const int tid = threadIdx.x;
+    const float *x = a.logits + (size_t)row * a.ld;
+    const float NaN = __uint_as_float(0x7fc00000u), ls = log1pf(t.s);
+    const bool bad = nan || !(t.m < INFINITY), none = t.m == -INFINITY;
+    auto lp = [&](float v) { return bad ? NaN : none ? -INFINITY : (v - t.m) - ls; };
+    if (tid == 0 && a.entropy) a.entropy[row] = bad ? NaN : none ? 0.0f : ls + t.d / (1.0f + t.s);
+    for (int g = tid; g < a.n_given; g += LP_BLOCK) {
+        const int id = a.given[(size_t)row * a.n_given + g];
+        a.logprob[(size_t)row * a.n_given + g] = id < 0 || id >= a.vocab ? NaN : lp(x[id]);
+    }
+    if (tid < a.top) {
+        const bool no = tid >= k;
+        a.top_id[(size_t)row * a.top + tid] = no || bad || none ? -1 : lp_index(key[tid]);
+        a.top_logprob[(size_t)row * a.top + tid] = bad ? NaN : no ? -INFINITY : lp(lp_value(key[tid]));
+    }
+}
+
+// A run of a row, runs side by side: `per` tiles of LP_BLOCK * E logits. Tiles start at the 16-byte
+// line of the row's first logit, so that every load but a row's first and last is whole.
+template <int E>
+__global__ __launch_bounds__(LP_BLOCK) void k_lp_run(LpArgs g) {
+    constexpr int TILE = LP_BLOCK * E, CAP = TILE + LP_LIST;
+    __shared__ LpList<CAP> l;
+    __shared__ float red[3 * LP_BLOCK / 64];
+    __shared__ __align__(16) float tops[LP_BLOCK];
+    __shared__ float bound;
+    const gmoe_logprobs_args &a = g.a;
+    const int tid = threadIdx.x, row = blockIdx.x / g.segs, seg = blockIdx.x - row * g.segs, V = a.vocab, top = a.top;
+    const float *x = a.logits + (size_t)row * a.ld;
+    const int lead = (int)((uintptr_t)x >> 2 & 3);  // logits of the first line before the row's
+    const int end = V + lead, i0 = seg * g.per * TILE, i1 = min(end, i0 + g.per * TILE);
+    const float *line = x - lead;
+    LpSum t = {-INFINITY, 0.0f, 0.0f};
+    bool nan = false;
+    float over = -INFINITY;  // a value passes above it
+    if (tid == 0) l.n = 0;
+    __syncthreads();
+    int n = 0;
+    for (int base = i0; base < i1; base += TILE) {
+        float v[E];
+        const bool edge = base < lead || base + TILE > end;
+#pragma unroll
+        for (int k = 0; k < E / 4; k++) {
+            const int i = base + 4 * (k * LP_BLOCK + tid);
+            if (!edge || (i >= lead && i + 4 <= end)) {
+                *(float4 *)&v[4 * k] = *(const float4 *)(line + i);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[4 * k + j] = i + j >= lead && i + j < end ? line[i + j] : -INFINITY;
+            }
+        }
+        float p[E];
+#pragma unroll
+        for (int k = 0; k < E; k++) {
+            p[k] = v[k];
+            nan |= v[k] != v[k];
+        }
+#pragma unroll
+        for (int w = E / 2; w >= 1; w >>= 1)
+#pragma unroll
+            for (int k = 0; k < w; k++) {
+                const float hi = fmaxf(p[k], p[k + w]), lo = fminf(p[k], p[k + w]);
+                p[k] = hi;
+                p[k + w] = lo;
+            }
+        const float tm = p[0], lo = fminf(t.m, tm), mn = fmaxf(t.m, tm), ref = fmaxf(mn, -FLT_MAX);
+        t.move(ref);
+        t.m = mn;
+        t.term(lo, ref);
+#pragma unroll
+        for (int k = 1; k < E; k++) t.term(p[k], ref);
+        if (top == 0) continue;
+        const bool first = base == i0;
+        if (first) {
+            // the top-th largest of the threads' maxima: as many values are no smaller
+            tops[tid] = tm;
+            __syncthreads();
+            int above = 0, equal = 0;
+            for (int j = 0; j < LP_BLOCK; j += 4) {
+                const float4 o = *(const float4 *)&tops[j];
+                above += (o.x > tm) + (o.y > tm) + (o.z > tm) + (o.w > tm);
+                equal += (o.x == tm) + (o.y == tm) + (o.z == tm) + (o.w == tm);
+            }
+            if (tid == 0) bound = -INFINITY;
+            __syncthreads();
+            if (above < top && above + equal >= top) bound = tm;
+            __syncthreads();
+            over = bound;
+        }
+        if (first ? tm >= over : tm > over) {
+#pragma unroll
+            for (int k = 0; k < E; k++) {
+                const int i = base + 4 * ((k >> 2) * LP_BLOCK + tid) + (k & 3);
+                if ((first ? v[k] >= over : v[k] > over) && i >= lead && i < end) l.key[atomicAdd(&l.n, 1u)] = lp_key(v[k], i - lead);
+            }
+        }
+        __syncthreads();
+        n = (int)l.n;
+        __syncthreads();
+        if (first || n > LP_CUT) {
+            n = lp_cut(l, n, top);
+            if (n == top) over = lp_value(l.key[top - 1]);
+            if (tid == 0) l.n = n;
+            __syncthreads();
         }
     }
+    nan = __syncthreads_or(nan);
+    t = lp_join(t, red);
+    if (top > 0) n = lp_cut(l, n, top);
+    if (g.segs == 1) {
+        lp_finish(a, row, t, nan, l.key, n);
+        return;
+    }
+    const size_t at = (size_t)row * g.segs + seg;
+    if (tid == 0) g.runs[at] = LpRun{t.m, t.s, t.d, nan ? -1 : n};
+    if (tid < n) g.keys[at * top + tid] = l.key[tid];
+}
+
+// A row's runs joined. Keys: those no smaller than the top-th largest of the runs' first keys, which
+// come from `top` runs at most.
+__global__ __launch_bounds__(LP_BLOCK) void k_lp_join(LpArgs g) {
+    constexpr int CAP = GMOE_TOP_MAX * GMOE_TOP_MAX;
+    __shared__ LpList<CAP> l;
+    __shared__ float red[3 * LP_BLOCK / 64];
+    __shared__ unsigned long long firsts[LP_SEGS];
+    __shared__ int counts[LP_SEGS];
+    __shared__ unsigned long long bound;
+    const int tid = threadIdx.x, row = blockIdx.x, top = g.a.top, segs = g.segs;
+    const size_t at = (size_t)row * segs;
+    LpSum t = {-INFINITY, 0.0f, 0.0f};
+    int n = 0;
+    if (tid < segs) {
+        const LpRun r = g.runs[at + tid];
+        t = {r.m, r.s, r.d};
+        n = r.n;
+    }
+    const bool nan = __syncthreads_or(n < 0);
+    t = lp_join(t, red);
+    if (top > 0) {
+        const unsigned long long mine = n > 0 ? g.keys[(at + tid) * top] : 0;
+        firsts[tid] = mine;
+        counts[tid] = max(n, 0);
+        if (tid == 0) {
+            bound = 0;
+            l.n = 0;
+        }
+        __syncthreads();
+        int above = 0;
+        for (int j = 0; j < segs; j++) above += firsts[j] > mine;
+        if (mine && above == top - 1) bound = mine;
+        __syncthreads();
+        const unsigned long long least = bound;
+        for (int i = tid; i < segs * top; i += LP_BLOCK) {
+            const int s = i / top;
+            if (i - s * top < counts[s] && firsts[s] >= least) {
+                const unsigned long long k = g.keys[at * top + i];
+                if (k >= least) l.key[atomicAdd(&l.n, 1u)] = k;
+            }
+        }
+        __syncthreads();
+        n = lp_cut(l, (int)l.n, top);
+    }
+    lp_finish(g.a, row, t, nan, l.key, n);
+}
+
+// How a call is split: tiles of 4096 logits where those make a block for every CU twice over,
+// else of 1024; then as many runs a row as keep LP_FILL blocks going.
+#define LP_FILL 2048
+struct LpSplit {
+    int e, segs, per;
+};
+static inline LpSplit lp_split(int n, int vocab) {
+    const long long want = (LP_FILL + (long long)n - 1) / n;  // runs a row
+    auto tiles = [&](int e) { return ((long long)vocab + 3 + LP_BLOCK * e - 1) / (LP_BLOCK * e); };
+    LpSplit s;
+    s.e = n * tiles(16) >= 512 ? 16 : 4;
+    const long long t = tiles(s.e);
+    const long long segs = std::max(1ll, std::min({t, want, (long long)LP_SEGS}));
+    s.per = (int)((t + segs - 1) / segs);
+    s.segs = (int)((t + s.per - 1) / s.per);
+    return s;
 }

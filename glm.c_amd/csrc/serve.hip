@@ -190,17 +190,16 @@ extern "C" int gmoe_kv4_attend(int device, const gmoe_kv4 *c, const gmoe_batch *
 }
 
 extern "C" size_t gmoe_logprobs_workspace(int n, int vocab, int top) {
-    (void)n;
-    (void)vocab;
-    (void)top;
-    return 0;
+    if (n < 1 || n > (1 << 24) || vocab < 1 || vocab > (1 << 24) || top < 0 || top > GMOE_TOP_MAX) return 0;
+    const LpSplit s = lp_split(n, vocab);
+    return s.segs > 1 ? (size_t)n * s.segs * (sizeof(LpRun) + top * sizeof(unsigned long long)) : 0;
 }
 
 extern "C" int gmoe_logprobs(int device, const gmoe_logprobs_args *a, void *stream) {
     if (!a) return invalid("gmoe_logprobs: null argument");
-    if (a->n < 0 || a->vocab < 1 || a->vocab > (1 << 24) || a->n_given < 0 || a->top < 0 || a->top > GMOE_TOP_MAX ||
+    if (a->n < 0 || a->n > (1 << 24) || a->vocab < 1 || a->vocab > (1 << 24) || a->n_given < 0 || a->top < 0 || a->top > GMOE_TOP_MAX ||
         (a->ld < a->vocab && a->n > 1))
-        return invalid("gmoe_logprobs: %lld rows of %lld logits, %lld given, %lld alternatives: outside 0.., 1..2^24, 0.., "
+        return invalid("gmoe_logprobs: %lld rows of %lld logits, %lld given, %lld alternatives: outside 0..2^24, 1..2^24, 0.., "
                        "0..64, or rows closer than that",
                        a->n, a->vocab, a->n_given, a->top);
     if (a->n == 0) return GMOE_OK;
@@ -213,7 +212,18 @@ extern "C" int gmoe_logprobs(int device, const gmoe_logprobs_args *a, void *stre
                        (long long)a->work_bytes);
     OnDevice on(device);
     if (on.err != hipSuccess) return failed("gmoe_logprobs: the device", on.err);
-    hipLaunchKernelGGL(k_logprobs, dim3((unsigned)a->n), dim3(LP_BLOCK), 0, (hipStream_t)stream, *a);
+    const LpSplit s = lp_split(a->n, a->vocab);
+    LpArgs g;
+    g.a = *a;
+    g.segs = s.segs;
+    g.per = s.per;
+    g.runs = (LpRun *)a->work;
+    g.keys = (unsigned long long *)(g.runs + (size_t)a->n * s.segs);
+    hipStream_t st = (hipStream_t)stream;
+    const dim3 grid((unsigned)a->n * (unsigned)s.segs);
+    if (s.e == 16) hipLaunchKernelGGL(k_lp_run<16>, grid, dim3(LP_BLOCK), 0, st, g);
+    else hipLaunchKernelGGL(k_lp_run<4>, grid, dim3(LP_BLOCK), 0, st, g);
+    if (s.segs > 1) hipLaunchKernelGGL(k_lp_join, dim3((unsigned)a->n), dim3(LP_BLOCK), 0, st, g);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? GMOE_OK : failed("gmoe_logprobs", e);
 }

@@ -131,7 +131,7 @@ size_t gmoe_kv4_attend_workspace(int n_heads, int kv_lora_rank);
 #define GMOE_TOP_MAX 64
 
 typedef struct gmoe_logprobs_args {
-    int32_t n, vocab;          /* rows (0 does nothing), columns 1..2^24 */
+    int32_t n, vocab;          /* rows 0..2^24 (0 does nothing), columns 1..2^24 */
     int32_t n_given, top;      /* given tokens (>= 0) and alternatives (0..GMOE_TOP_MAX) a row */
     const float *logits;       /* row i: logits + i * ld, ld >= vocab floats */
     int64_t ld;

@@ -111,7 +111,7 @@ def test_attend_refuses(over):
         c.attend(batch(**{k: v for k, v in over.items() if k not in a}), **a)
 
 
-@pytest.mark.parametrize("over", [dict(n=-1), dict(vocab=0), dict(vocab=(1 << 24) + 1), dict(top=-1), dict(top=65), dict(n_given=-1),
+@pytest.mark.parametrize("over", [dict(n=-1), dict(n=(1 << 24) + 1), dict(vocab=0), dict(vocab=(1 << 24) + 1), dict(top=-1), dict(top=65), dict(n_given=-1),
                                   dict(ld=99), dict(logits=None), dict(logits=HERE + 2), dict(given=None), dict(logprob=None),
                                   dict(top_id=None), dict(top_logprob=None)])
 def test_logprobs_refuses(over):
@@ -121,6 +121,14 @@ def test_logprobs_refuses(over):
     a.update({k: v for k, v in over.items() if k in a})
     with pytest.raises(RuntimeError, match=r"gmoe_logprobs failed \(-1\)"):
         gmoe.LogProbs(**s)(**a)
+
+
+def test_a_short_workspace_is_refused():
+    lp = gmoe.LogProbs(1, 154880, 20, 1)  # one row over the whole GPU
+    assert lp.workspace > 0
+    for work, size in ((HERE, lp.workspace - 1), (None, lp.workspace), (HERE + 8, lp.workspace)):
+        with pytest.raises(RuntimeError, match="workspace"):
+            lp(HERE, 154880, HERE, HERE, None, HERE, HERE, work, size)
 
 
 def test_sizes():
