@@ -11,9 +11,9 @@
 //
 // Top alternatives. Keys order the logits by value, then the lower index, and no two are
 // equal. A block keeps the list of keys that may be among its `top` largest: those above a
-// threshold, which starts as the top-th largest of the first tile's per-thread maxima (at least
-// `top` values are no smaller) and is set to the list's top-th key each time the list is cut
-// to `top`. After the first tiles nearly no value passes, so that a tile costs one comparison a
+// threshold, which starts from the first tile's per-thread maxima (a value that `top` of them reach,
+// a quarter in each wave) and is set to the list's top-th key each time the list is cut to
+// `top`. After the first tiles nearly no value passes, so that a tile costs one comparison a
 // thread. Later tiles hold higher indexes, so a value equal to the threshold does not pass.
 //
 // Split. A block takes a run of tiles of a row; with more than one run a row (few rows) the
@@ -27,9 +27,12 @@
 #include "pages.h"
 
 #define LP_BLOCK 256
+#define LP_E 8           // logits a thread holds: with 16, half the blocks fit a CU (801 rows: 117 us against 98)
+#define LP_TILE (LP_BLOCK * LP_E)
 #define LP_SEGS 256     // most runs of a row: a thread each in k_lp_join
-#define LP_LIST 512     // list entries besides a tile's
+#define LP_LIST 192     // list entries besides a tile's (LP_CUT and more: eight blocks' shared memory fits a CU)
 #define LP_CUT 160      // the list is cut to `top` when it is longer
+static_assert(LP_LIST >= LP_CUT && LP_CUT >= GMOE_TOP_MAX, "a tile's values fit behind a list that is not cut");
 
 // A run's result: the triple, its keys' number, whether a value is NaN.
 struct LpRun {
@@ -75,13 +78,17 @@ struct LpSum {
     }
 };
 
+// Sum over the 64 lanes of a wave, to every lane.
+__device__ static inline float wave_sum_dpp_f(float v) {
+    v = row_sum_dpp_f(v);
+    return (readlane_f(v, 0) + readlane_f(v, 16)) + (readlane_f(v, 32) + readlane_f(v, 48));
+}
+
 // The block's triples joined into one, in every thread; red: 3 * LP_BLOCK / 64 floats.
 __device__ static inline LpSum lp_join(LpSum v, float *red) {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     constexpr int W = LP_BLOCK / 64;
-    float M = v.m;
-#pragma unroll
-    for (int k = 32; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor(M, k));
+    float M = wave_max_dpp_f(v.m);
     __syncthreads();
     if (lane == 0) red[w] = M;
     __syncthreads();
@@ -94,11 +101,8 @@ __device__ static inline LpSum lp_join(LpSum v, float *red) {
     const float ref = fmaxf(M, -FLT_MAX), m0 = v.m;
     v.move(ref);
     if (!mine) v.term(m0, ref);
-#pragma unroll
-    for (int k = 32; k > 0; k >>= 1) {
-        v.s += __shfl_xor(v.s, k);
-        v.d += __shfl_xor(v.d, k);
-    }
+    v.s = wave_sum_dpp_f(v.s);
+    v.d = wave_sum_dpp_f(v.d);
     if (lane == 0) {
         red[W + w] = v.s;
         red[2 * W + w] = v.d;
@@ -168,10 +172,17 @@ __device__ static int lp_cut(LpList<CAP> &l, int n, int top) {
     // ranked by counting the larger ones
     const unsigned long long k0 = tid < n ? src[tid] : 0, k1 = tid + LP_BLOCK < n ? src[tid + LP_BLOCK] : 0;
     int r0 = 0, r1 = 0;
-    for (int j = 0; j < n; j++) {
-        const unsigned long long k = src[j];
-        r0 += k > k0;
-        r1 += k > k1;
+    if (n <= LP_BLOCK) {
+        if ((tid & ~63) < n)  // (the other waves hold none)
+#pragma unroll 8
+            for (int j = 0; j < n; j++) r0 += src[j] > k0;
+    } else {
+#pragma unroll 8
+        for (int j = 0; j < n; j++) {
+            const unsigned long long k = src[j];
+            r0 += k > k0;
+            r1 += k > k1;
+        }
     }
     __syncthreads();
     if (tid < n && r0 < top) l.key[r0] = k0;
@@ -180,19 +191,23 @@ __device__ static int lp_cut(LpList<CAP> &l, int n, int top) {
     return min(n, top);
 }
 
-// The row's results from its joined triple and its alternatives (k of them, the largest first).
+// The logit of the row's given token g, NaN outside the vocabulary.
+__device__ static inline float lp_given(const gmoe_logprobs_args &a, int row, int g) {
+    const int id = a.given[(size_t)row * a.n_given + g];
+    return id < 0 || id >= a.vocab ? __uint_as_float(0x7fc00000u) : a.logits[(size_t)row * a.ld + id];
+}
+
+// The row's results from its joined triple and its alternatives (k of them, the largest first);
+// given: the thread's lp_given of the first LP_BLOCK tokens, requested long before.
 __device__ static inline void lp_finish(const gmoe_logprobs_args &a, int row, const LpSum &t, bool nan, const unsigned long long *key,
-                                        int k) {
+                                        int k, float given) {
     const int tid = threadIdx.x;
-    const float *x = a.logits + (size_t)row * a.ld;
     const float NaN = __uint_as_float(0x7fc00000u), ls = log1pf(t.s);
     const bool bad = nan || !(t.m < INFINITY), none = t.m == -INFINITY;
-    auto lp = [&](float v) { return bad ? NaN : none ? -INFINITY : (v - t.m) - ls; };
+    auto lp = [&](float v) { return bad || v != v ? NaN : none ? -INFINITY : (v - t.m) - ls; };
     if (tid == 0 && a.entropy) a.entropy[row] = bad ? NaN : none ? 0.0f : ls + t.d / (1.0f + t.s);
-    for (int g = tid; g < a.n_given; g += LP_BLOCK) {
-        const int id = a.given[(size_t)row * a.n_given + g];
-        a.logprob[(size_t)row * a.n_given + g] = id < 0 || id >= a.vocab ? NaN : lp(x[id]);
-    }
+    for (int g = tid; g < a.n_given; g += LP_BLOCK)
+        a.logprob[(size_t)row * a.n_given + g] = lp(g == tid ? given : lp_given(a, row, g));
     if (tid < a.top) {
         const bool no = tid >= k;
         a.top_id[(size_t)row * a.top + tid] = no || bad || none ? -1 : lp_index(key[tid]);
@@ -200,15 +215,13 @@ __device__ static inline void lp_finish(const gmoe_logprobs_args &a, int row, co
     }
 }
 
-// A run of a row, runs side by side: `per` tiles of LP_BLOCK * E logits. Tiles start at the 16-byte
+// A run of a row, runs side by side: `per` tiles of LP_TILE logits. Tiles start at the 16-byte
 // line of the row's first logit, so that every load but a row's first and last is whole.
-template <int E>
-__global__ __launch_bounds__(LP_BLOCK) void k_lp_run(LpArgs g) {
-    constexpr int TILE = LP_BLOCK * E, CAP = TILE + LP_LIST;
-    __shared__ LpList<CAP> l;
+__global__ __launch_bounds__(LP_BLOCK, 8) void k_lp_run(LpArgs g) {
+    constexpr int E = LP_E, TILE = LP_TILE;
+    __shared__ LpList<TILE + LP_LIST> l;
     __shared__ float red[3 * LP_BLOCK / 64];
-    __shared__ __align__(16) float tops[LP_BLOCK];
-    __shared__ float bound;
+    __shared__ float tops[LP_BLOCK / 64];
     const gmoe_logprobs_args &a = g.a;
     const int tid = threadIdx.x, row = blockIdx.x / g.segs, seg = blockIdx.x - row * g.segs, V = a.vocab, top = a.top;
     const float *x = a.logits + (size_t)row * a.ld;
@@ -216,11 +229,12 @@ __global__ __launch_bounds__(LP_BLOCK) void k_lp_run(LpArgs g) {
     const int end = V + lead, i0 = seg * g.per * TILE, i1 = min(end, i0 + g.per * TILE);
     const float *line = x - lead;
     LpSum t = {-INFINITY, 0.0f, 0.0f};
+    const float given = g.segs == 1 && tid < a.n_given ? lp_given(a, row, tid) : 0.0f;
     bool nan = false;
     float over = -INFINITY;  // a value passes above it
     if (tid == 0) l.n = 0;
     __syncthreads();
-    int n = 0;
+    int n = 0, cut = 0;  // the list's length, and what it was cut to
     for (int base = i0; base < i1; base += TILE) {
         float v[E];
         const bool edge = base < lead || base + TILE > end;
@@ -257,20 +271,16 @@ __global__ __launch_bounds__(LP_BLOCK) void k_lp_run(LpArgs g) {
         if (top == 0) continue;
         const bool first = base == i0;
         if (first) {
-            // the top-th largest of the threads' maxima: as many values are no smaller
-            tops[tid] = tm;
-            __syncthreads();
-            int above = 0, equal = 0;
-            for (int j = 0; j < LP_BLOCK; j += 4) {
-                const float4 o = *(const float4 *)&tops[j];
-                above += (o.x > tm) + (o.y > tm) + (o.z > tm) + (o.w > tm);
-                equal += (o.x == tm) + (o.y == tm) + (o.z == tm) + (o.w == tm);
+            // a value that a quarter of `top` of each wave's maxima reach, so that `top` values do
+            const int quarter = (top + LP_BLOCK / 64 - 1) / (LP_BLOCK / 64);
+            float best = wave_max_dpp_f(tm), rest = tm;
+            for (int j = 1; j < quarter; j++) {  // the largest below the ones before, of which there was one at least each
+                rest = rest < best ? rest : -INFINITY;
+                best = wave_max_dpp_f(rest);
             }
-            if (tid == 0) bound = -INFINITY;
+            if ((tid & 63) == 0) tops[tid >> 6] = best;
             __syncthreads();
-            if (above < top && above + equal >= top) bound = tm;
-            __syncthreads();
-            over = bound;
+            over = fminf(fminf(tops[0], tops[1]), fminf(tops[2], tops[3]));
         }
         if (first ? tm >= over : tm > over) {
 #pragma unroll
@@ -279,11 +289,11 @@ __global__ __launch_bounds__(LP_BLOCK) void k_lp_run(LpArgs g) {
                 if ((first ? v[k] >= over : v[k] > over) && i >= lead && i < end) l.key[atomicAdd(&l.n, 1u)] = lp_key(v[k], i - lead);
             }
         }
-        __syncthreads();
+        block_barrier();
         n = (int)l.n;
-        __syncthreads();
+        block_barrier();
         if (first || n > LP_CUT) {
-            n = lp_cut(l, n, top);
+            n = cut = lp_cut(l, n, top);
             if (n == top) over = lp_value(l.key[top - 1]);
             if (tid == 0) l.n = n;
             __syncthreads();
@@ -291,9 +301,9 @@ __global__ __launch_bounds__(LP_BLOCK) void k_lp_run(LpArgs g) {
     }
     nan = __syncthreads_or(nan);
     t = lp_join(t, red);
-    if (top > 0) n = lp_cut(l, n, top);
+    if (n > cut) n = lp_cut(l, n, top);
     if (g.segs == 1) {
-        lp_finish(a, row, t, nan, l.key, n);
+        lp_finish(a, row, t, nan, l.key, n, given);
         return;
     }
     const size_t at = (size_t)row * g.segs + seg;
@@ -308,60 +318,61 @@ __global__ __launch_bounds__(LP_BLOCK) void k_lp_join(LpArgs g) {
     __shared__ LpList<CAP> l;
     __shared__ float red[3 * LP_BLOCK / 64];
     __shared__ unsigned long long firsts[LP_SEGS];
-    __shared__ int counts[LP_SEGS];
+    __shared__ int counts[LP_SEGS], from[GMOE_TOP_MAX];
     __shared__ unsigned long long bound;
     const int tid = threadIdx.x, row = blockIdx.x, top = g.a.top, segs = g.segs;
     const size_t at = (size_t)row * segs;
     LpSum t = {-INFINITY, 0.0f, 0.0f};
     int n = 0;
+    unsigned long long mine = 0;
+    const float given = tid < g.a.n_given ? lp_given(g.a, row, tid) : 0.0f;
     if (tid < segs) {
         const LpRun r = g.runs[at + tid];
+        if (top > 0) mine = g.keys[(at + tid) * top];
         t = {r.m, r.s, r.d};
         n = r.n;
+        mine = n > 0 ? mine : 0;
     }
     const bool nan = __syncthreads_or(n < 0);
     t = lp_join(t, red);
     if (top > 0) {
-        const unsigned long long mine = n > 0 ? g.keys[(at + tid) * top] : 0;
         firsts[tid] = mine;
         counts[tid] = max(n, 0);
         if (tid == 0) {
-            bound = 0;
             l.n = 0;
+            bound = 0;
         }
         __syncthreads();
-        int above = 0;
+        int above = 0;  // runs with a larger first key
+#pragma unroll 8
         for (int j = 0; j < segs; j++) above += firsts[j] > mine;
+        if (mine && above < top) from[above] = tid;
         if (mine && above == top - 1) bound = mine;
-        __syncthreads();
+        const int live = min(top, __syncthreads_count(mine != 0));
         const unsigned long long least = bound;
-        for (int i = tid; i < segs * top; i += LP_BLOCK) {
-            const int s = i / top;
-            if (i - s * top < counts[s] && firsts[s] >= least) {
-                const unsigned long long k = g.keys[at * top + i];
-                if (k >= least) l.key[atomicAdd(&l.n, 1u)] = k;
-            }
+#pragma unroll 2
+        for (int i = tid; i < live * top; i += LP_BLOCK) {
+            const int s = from[i / top], j = i % top;
+            const unsigned long long k = j < counts[s] ? g.keys[(at + s) * top + j] : 0;
+            if (k && k >= least) l.key[atomicAdd(&l.n, 1u)] = k;
         }
         __syncthreads();
         n = lp_cut(l, (int)l.n, top);
     }
-    lp_finish(g.a, row, t, nan, l.key, n);
+    lp_finish(g.a, row, t, nan, l.key, n, given);
 }
 
-// How a call is split: tiles of 4096 logits where those make a block for every CU twice over,
-// else of 1024; then as many runs a row as keep LP_FILL blocks going.
+// How a call is split: as many runs a row as the GPU holds at once (eight blocks a CU), so that
+// every block starts at once and none is left for a second turn. 801 rows of 151551 (1602 blocks):
+// 98 us, and 113 with 2403 blocks, 139 with 801; 64 rows of 154880: 17 us with 26 runs a row, 20 with 13.
 #define LP_FILL 2048
 struct LpSplit {
-    int e, segs, per;
+    int segs, per;  // runs a row, tiles a run
 };
 static inline LpSplit lp_split(int n, int vocab) {
-    const long long want = (LP_FILL + (long long)n - 1) / n;  // runs a row
-    auto tiles = [&](int e) { return ((long long)vocab + 3 + LP_BLOCK * e - 1) / (LP_BLOCK * e); };
+    const int tiles = (vocab + 3 + LP_TILE - 1) / LP_TILE, want = std::max(1, std::min({tiles, LP_FILL / n, LP_SEGS}));
     LpSplit s;
-    s.e = n * tiles(16) >= 512 ? 16 : 4;
-    const long long t = tiles(s.e);
-    const long long segs = std::max(1ll, std::min({t, want, (long long)LP_SEGS}));
-    s.per = (int)((t + segs - 1) / segs);
-    s.segs = (int)((t + s.per - 1) / s.per);
+    s.per = (tiles + want - 1) / want;
+    s.segs = (tiles + s.per - 1) / s.per;
     return s;
 }

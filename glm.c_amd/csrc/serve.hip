@@ -221,8 +221,7 @@ extern "C" int gmoe_logprobs(int device, const gmoe_logprobs_args *a, void *stre
     g.keys = (unsigned long long *)(g.runs + (size_t)a->n * s.segs);
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)a->n * (unsigned)s.segs);
-    if (s.e == 16) hipLaunchKernelGGL(k_lp_run<16>, grid, dim3(LP_BLOCK), 0, st, g);
-    else hipLaunchKernelGGL(k_lp_run<4>, grid, dim3(LP_BLOCK), 0, st, g);
+    hipLaunchKernelGGL(k_lp_run, grid, dim3(LP_BLOCK), 0, st, g);
     if (s.segs > 1) hipLaunchKernelGGL(k_lp_join, dim3((unsigned)a->n), dim3(LP_BLOCK), 0, st, g);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? GMOE_OK : failed("gmoe_logprobs", e);
