@@ -25,7 +25,6 @@
                             // k_attn_tile16's longest-first order, 3 beat 5 by ~1 %: fewer partial results)
 #define AQ_SLOTS (AQ_P * (AQ_KQ_MAX / 4 + 1) + 64)  // 16-byte slots of a stage (one wave's DMA past the rows)
 
-typedef float aq_f4 __attribute__((ext_vector_type(4)));
 
 struct AttnTileArgs {
     AttnArgs a;  // a.pos = the batch's first position, a.nblk = chunks per token

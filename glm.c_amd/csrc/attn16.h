@@ -74,18 +74,6 @@ constexpr bool a16_scale_bounded() {
 }
 static_assert(a16_scale_bounded(), "a step down lands on the tile's exponent or on the sum's bound");
 
-typedef _Float16 a16_h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 a16_h4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) a16_h4 a16_lds_h4;
-
-// The 16-lane group's 4 rows x 16 columns of halves, transposed: lane i of the group names
-// the 8 bytes at row i / 4, columns 4 (i % 4) .. + 3, and gets column i of the four rows.
-__device__ static inline a16_h4 a16_tr(const _Float16 *p) {
-    typedef short s4 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) s4 lds_s4;
-    return __builtin_bit_cast(a16_h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)p));
-}
-
 // The maximum over the four lanes l % 16 + {0, 16, 32, 48}.
 __device__ static inline float a16_max4(float v) {
     typedef unsigned u2 __attribute__((ext_vector_type(2)));

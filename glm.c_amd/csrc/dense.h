@@ -7,6 +7,7 @@
 #pragma once
 
 #include "common.h"
+#include "split16.h"
 
 #define DM_BLOCK 256
 
@@ -254,22 +255,7 @@ struct AttnArgs {
 #define SPL_KCOLS 576
 #define SPL_KEXP (2 * SPL_KCOLS)   // half index of the exponent in a ksp row
 #define SPL_KROW (2 * SPL_KCOLS + 16)
-#define SPL_EMPTY (-1000)
 static_assert(SPL_KROW * 2 % 256 == 32 && SPL_KROW * 2 % 16 == 0, "ksp rows lie 8 banks apart");
-
-// The exponent e with |x| 2^-e < 2^15 for every |x| <= mx (SPL_EMPTY when mx is 0).
-__device__ static inline int spl_exp(float mx) {
-    if (!(mx > 0.0f)) return SPL_EMPTY;
-    int k;
-    (void)frexpf(mx, &k);  // mx < 2^k
-    return k - 15;
-}
-
-// x = hi + lo: hi the nearest fp16, lo the nearest fp16 to the (exact) remainder.
-__device__ static inline void spl_split(float x, _Float16 &hi, _Float16 &lo) {
-    hi = (_Float16)x;
-    lo = (_Float16)(x - (float)hi);
-}
 
 // The split form of the entry row[0 .. kv + rope) (the block's shared memory, written before
 // a barrier) into ksp row kr (kv + rope <= SPL_KCOLS: the host's check); rmax: DM_BLOCK / 64

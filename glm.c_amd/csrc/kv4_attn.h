@@ -1,21 +1,55 @@
 // kv4_attn.h -- MLA attention of a step's tokens over the paged cache in 4 bits (gmoe_kv4_attend).
 //
-// Work split. A request's fresh tokens times heads are its query rows; a tile is KA_ROWS of them,
-// and an item is a tile against a chunk of the request's positions. All chunks of a launch are
-// one length, a multiple of KA_UNIT positions, the least that makes at most KA_ITEMS items beside
-// the one a tile needs (kv4_plan): few long requests are cut fine, many are not cut at all. The
-// lengths are device data, so every block works out the split by itself, from the requests'
+// Work split. A request's fresh tokens times heads are its query rows; a tile is 8 MT of them
+// (MT 1, 2 or 3), and an item is a tile against a chunk of the request's positions. All chunks of a launch are
+// one length, a multiple of KA_P positions, the least that makes at most KA_ITEMS items beside
+// the one a tile needs (ka_plan): few long requests are cut fine, many are not cut at all. The
+// lengths are device data, so every block works out the split by itself from the requests'
 // lengths, and the grid is a fixed number of blocks that walk the items. A tile of one chunk is
 // written where it belongs; the others leave partial results that k_kv4_merge joins.
+//
+// Products. Both run on v_mfma_f32_16x16x32_f16. The cache's values are exact in fp16 (e2m1 times a
+// power of two that the format holds to fp16's range), so only the queries and the exponentials
+// are split into two fp16 parts, x = hi + lo to 22 bits: two products where split operands on both sides
+// take three. The two parts of eight rows make the 16 operand rows of a tile, in the order
+// (hi hi lo lo) of rows 2g, 2g + 1: then a row's two sums lie in the same lane.
+//
+// A block (8 waves, one a CU) takes KA_P = 64 positions at a time:
+//   scores   wave (h, g) has half h of the columns (nine blocks of 32) and positions 16 g .. + 15. A lane
+//            loads 16 bytes, a block of 32 codes, which are four steps' operands when the steps run over
+//            the blocks' eighths (the sum over columns may run in any order); v_cvt_scalef32_pk_f16_fp4
+//            turns a byte of codes and their scale into two halves. The queries stay in registers
+//            (108). The halves go to shared memory as they are, a row a position.
+//   softmax  wave w has rows 3 w .. + 2, a lane a position; the exponentials go to shared memory as
+//            operands.
+//   values   wave w has columns 64 w .. + 63: the rows of halves through the transposing read.
+// The values of a tile and the scores of the next share a phase, so two barriers a tile; codes
+// are requested a tile ahead, pages two.
+//
+// Softmax reference: exponentials are taken against a row's reference, which follows the running
+// maximum only when a score passes it by 2^KA_SLACK, so that sums are rescaled a few times a
+// chunk. They are scaled by 2^KA_UP for the split, whose error is then 2^-33 of the largest.
 #pragma once
 
 #include "kv4.h"
+#include "split16.h"
 
-#define KA_ROWS 24
-#define KA_UNIT 64
+#define KA_P 64
+#define KA_BLOCK 512
+#define KA_WAVES (KA_BLOCK / 64)
+#define KA_ROWS 24    // rows of the largest tile
+#define KA_HALF 9     // column blocks of a wave's half
+#define KA_GRID 256
 #define KA_ITEMS 512
 #define KA_MAX_PARTS (2 * KA_ITEMS)  // a cut tile has over U/c + 1 <= 2 U/c chunks, U/c of all at most KA_ITEMS
-#define KA_BLOCK 256
+#define KA_SLACK 6.0f
+#define KA_UP 8
+#define KA_VROW 528  // halves of a row of values in shared memory: rows 8 banks apart (of 64)
+#define KA_SROW 26   // floats of a position's scores
+#define KA_PROW 72   // halves of an operand row of exponentials
+#define KA_QROW 584  // halves of an operand row of queries (while they are staged)
+static_assert(2 * KA_HALF >= KV4_BLOCKS_MAX, "two halves hold a row");
+static_assert(2 * KA_ROWS * KA_QROW <= 2 * KA_P * KA_VROW, "the queries are staged where the values come later");
 
 struct Kv4Attn {
     Kv4Cache c;
@@ -26,256 +60,475 @@ struct Kv4Attn {
     int64_t ld_q_abs, ld_q_pe, ld_out;
     float *out;
     float *part;     // [KA_MAX_PARTS][KA_ROWS][kv]
-    float *part_ml;  // [KA_MAX_PARTS][KA_ROWS][2]: a chunk's largest score and its sum of exponentials
+    float *part_ml;  // [KA_MAX_PARTS][KA_ROWS][2]: a chunk's reference (of base 2) and its sum of exponentials
 };
 
-// The split of a launch, in shared memory.
-struct Kv4Plan {
-    unsigned items[PM_MAX_R];  // items up to and with the request
-    unsigned parts[PM_MAX_R];  // partial results before the request
-    unsigned red[KA_BLOCK / 64];
-    unsigned long long red2[KA_BLOCK / 64];
-    unsigned total, chunk;  // items; units of a chunk
-};
+// ---- the split of a launch -------------------------------------------------------------------
 
-__device__ static inline unsigned ka_tiles(const Kv4Attn &a, int r) {
+__device__ static inline unsigned ka_tiles(const Kv4Attn &a, int r, int rows) {
     const int fresh = a.offsets[r + 1] - a.offsets[r];
-    return fresh > 0 ? (unsigned)(((long long)fresh * a.H + KA_ROWS - 1) / KA_ROWS) : 0u;
+    return fresh > 0 ? (unsigned)(fresh * a.H + rows - 1) / rows : 0u;  // (fresh * H < 2^27)
 }
 __device__ static inline unsigned ka_units(const Kv4Attn &a, int r) {
     const long long n = min((long long)a.context[r], (long long)a.max_pages << a.c.shift);  // what the table names
-    return n > 0 ? ((unsigned)n + KA_UNIT - 1) / KA_UNIT : 0u;
+    return n > 0 ? ((unsigned)n + KA_P - 1) / KA_P : 0u;
 }
 
-__device__ static inline void kv4_plan(const Kv4Attn &a, Kv4Plan &p) {
-    const int tid = threadIdx.x, R = a.R, per = (R + KA_BLOCK - 1) / KA_BLOCK, r0 = tid * per, r1 = min(R, r0 + per);
+// A thread's share of the requests, and what lies before it. Cut tiles are those of more than one chunk.
+struct KaPlan {
+    int r0, r1;
+    unsigned items0, items, cuts0, cuts, parts0;
+    unsigned chunk, total, total_cuts;  // units of a chunk; all items; all cut tiles
+};
+struct KaShared {
+    unsigned red[KA_WAVES];
+    unsigned long long red2[KA_WAVES];
+};
+
+__device__ static inline unsigned ka_chunks(unsigned units, unsigned chunk) { return max(1u, (units + chunk - 1) / chunk); }
+
+__device__ static inline KaPlan ka_plan(const Kv4Attn &a, int rows, KaShared &sh) {
+    const int tid = threadIdx.x, nw = blockDim.x >> 6, per = (a.R + blockDim.x - 1) / blockDim.x;
+    KaPlan p;
+    p.r0 = min(a.R, tid * per);
+    p.r1 = min(a.R, p.r0 + per);
     unsigned long long work = 0;
-    for (int r = r0; r < r1; r++) work += (unsigned long long)ka_tiles(a, r) * ka_units(a, r);
+    for (int r = p.r0; r < p.r1; r++) work += (unsigned long long)ka_tiles(a, r, rows) * ka_units(a, r);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) work += __shfl_xor(work, d);
-    if ((tid & 63) == 0) p.red2[tid >> 6] = work;
+    if ((tid & 63) == 0) sh.red2[tid >> 6] = work;
     __syncthreads();
     work = 0;
-    for (int i = 0; i < KA_BLOCK / 64; i++) work += p.red2[i];
-    const unsigned chunk = (unsigned)max(1ull, min((work + KA_ITEMS - 1) / KA_ITEMS, 1ull << 30));
-    unsigned items = 0, parts = 0;
-    for (int r = r0; r < r1; r++) {
-        const unsigned t = ka_tiles(a, r), k = max(1u, (ka_units(a, r) + chunk - 1) / chunk);
-        items += t * k;
-        if (k > 1) parts += t * k;
+    for (int i = 0; i < nw; i++) work += sh.red2[i];
+    p.chunk = (unsigned)max(1ull, min((work + KA_ITEMS - 1) / KA_ITEMS, 1ull << 30));
+    p.items = p.cuts = 0;
+    unsigned parts = 0;
+    for (int r = p.r0; r < p.r1; r++) {
+        const unsigned t = ka_tiles(a, r, rows), k = ka_chunks(ka_units(a, r), p.chunk);
+        p.items += t * k;
+        if (k > 1) {
+            p.cuts += t;
+            parts += t * k;
+        }
     }
-    unsigned n, np;
-    unsigned i0 = block_scan_u(items, p.red, &n), p0 = block_scan_u(parts, p.red, &np);
-    for (int r = r0; r < r1; r++) {
-        const unsigned t = ka_tiles(a, r), k = max(1u, (ka_units(a, r) + chunk - 1) / chunk);
-        i0 += t * k;
-        p.items[r] = i0;
-        p.parts[r] = p0;
-        if (k > 1) p0 += t * k;
-    }
-    if (tid == 0) {
-        p.total = n;
-        p.chunk = chunk;
-    }
-    __syncthreads();
+    unsigned n;
+    p.items0 = block_scan_u(p.items, sh.red, &p.total);
+    p.cuts0 = block_scan_u(p.cuts, sh.red, &p.total_cuts);
+    p.parts0 = block_scan_u(parts, sh.red, &n);
+    return p;
 }
 
 // One item of the split.
-struct Kv4Item {
+struct KaItem {
     int r, tile, k, chunk;     // request, tile of it, its chunks, this one
     int t0, fresh, context;    // the request's first token, its tokens, its positions
-    int s0, s1;                // positions of the chunk that any row of the tile attends
-    unsigned part;             // partial-result slot (k > 1)
+    unsigned part;             // partial-result slot of the item (k > 1)
 };
-__device__ static inline Kv4Item kv4_item(const Kv4Attn &a, const Kv4Plan &p, unsigned i) {
-    Kv4Item m;
-    m.r = upper_bound_u(p.items, a.R, i);
-    const unsigned local = i - (m.r > 0 ? p.items[m.r - 1] : 0u);
-    m.k = (int)max(1u, (ka_units(a, m.r) + p.chunk - 1) / p.chunk);
-    m.tile = (int)(local / m.k);
-    m.chunk = (int)(local % m.k);
-    m.part = p.parts[m.r] + local;
-    m.t0 = a.offsets[m.r];
-    m.fresh = a.offsets[m.r + 1] - m.t0;
-    m.context = max(0, a.context[m.r]);
-    const int last = min(m.fresh - 1, (int)(((long long)(m.tile + 1) * KA_ROWS - 1) / a.H));  // the tile's last token
-    const long long c0 = (long long)m.chunk * p.chunk * KA_UNIT, c1 = c0 + (long long)p.chunk * KA_UNIT;
-    const int end = (int)min((long long)max(0, m.context - m.fresh + last + 1), (long long)a.max_pages << a.c.shift);
-    m.s0 = (int)min(c0, (long long)end);
-    m.s1 = (int)min(c1, (long long)end);
-    return m;
+
+// The item of number `i` (of the cut tiles, first chunk, when CUT) by the thread that has it.
+template <bool CUT>
+__device__ static inline void ka_find(const Kv4Attn &a, const KaPlan &p, int rows, unsigned i, KaItem *out) {
+    const unsigned base = CUT ? p.cuts0 : p.items0, mine = CUT ? p.cuts : p.items;
+    if (i - base >= mine) return;
+    unsigned left = i - base, part = p.parts0;
+    for (int r = p.r0; r < p.r1; r++) {
+        const unsigned t = ka_tiles(a, r, rows), k = ka_chunks(ka_units(a, r), p.chunk), n = CUT ? (k > 1 ? t : 0) : t * k;
+        if (left < n) {
+            KaItem m;
+            m.r = r;
+            m.k = (int)k;
+            m.tile = (int)(CUT ? left : left / k);
+            m.chunk = (int)(CUT ? 0 : left % k);
+            m.t0 = a.offsets[r];
+            m.fresh = a.offsets[r + 1] - m.t0;
+            m.context = max(0, a.context[r]);
+            m.part = part + m.tile * k + m.chunk;
+            *out = m;
+            return;
+        }
+        left -= n;
+        if (k > 1) part += t * k;
+    }
 }
 
-// A plain form for any shape: a tile's queries and 32 positions' values in shared memory in fp32.
-#define KS_P 32
-#define KS_LD (KV4_BLOCKS_MAX * 32 + 4)
-__global__ __launch_bounds__(KA_BLOCK) void k_kv4_attend(Kv4Attn a) {
-    __shared__ Kv4Plan plan;
-    __shared__ float q[KA_ROWS][KS_LD];
-    __shared__ float kt[KS_P / 2][KS_LD];
-    __shared__ float sc[KA_ROWS][KS_P / 2];
-    __shared__ float ml[KA_ROWS][2], cr[KA_ROWS];
-    __shared__ int on[KS_P / 2];
-    constexpr int P = KS_P / 2;
-    const int tid = threadIdx.x, kv = a.c.kv, rope = a.c.rope, cols = 32 * a.c.blocks, lanes = 4 * a.c.blocks;
-    kv4_plan(a, plan);
+// ---- the kernel ------------------------------------------------------------------------------
+
+typedef _Float16 ka_h2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+// Eight codes and their scale to eight halves.
+__device__ static inline a16_h8 ka_halves(unsigned codes, float scale) {
+    const ka_h2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 1);
+    const ka_h2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3);
+    return (a16_h8){a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// The codes and scales of a lane's position and half, as loaded.
+struct KaRaw {
+    u32x4 q0, q1;  // blocks j and 4 + j of the half (j = lane / 16)
+    unsigned q2;   // the lane's eighth of block 8
+    unsigned w0, w1, w2;  // the half's scale bytes, from byte 0 (first half) or 1 on
+    bool on;
+};
+
+template <int MT>
+__global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
+    constexpr int ROWS = 8 * MT, OPS = 16 * MT, RPW = MT;  // rows, operand rows, rows of a wave's softmax
+    static_assert(RPW * KA_WAVES == ROWS, "every row has a wave");
+    __shared__ __align__(16) _Float16 val[2][KA_P * KA_VROW];
+    __shared__ __align__(16) float sc[2][KA_P][KA_SROW];
+    __shared__ __align__(16) _Float16 pr[OPS][KA_PROW];
+    __shared__ float cr[ROWS], rl[ROWS], rm[ROWS];
+    __shared__ int moved[KA_WAVES];
+    __shared__ KaShared sh;
+    __shared__ KaItem item;
+    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), kh = w >> 2, pg = w & 3;
+    const int kv = a.c.kv, rope = a.c.rope, nb = a.c.blocks, shift = a.c.shift;
+    const KaPlan plan = ka_plan(a, ROWS, sh);
+    const float L = 1.44269504f;
+    // the lane's blocks of its half, and where their scales lie in the half's bytes
+    const int b0 = KA_HALF * kh + lg, b1 = b0 + 4, b2 = KA_HALF * kh + 8;
+    const unsigned none = 0x0c0c0c0cu, sel0 = b0 < nb ? 0x0c0c0c00u + kh + lg : none, sel1 = b1 < nb ? 0x0c0c0c00u + kh + lg : none,
+                   sel2 = b2 < nb ? 0x0c0c0c00u + kh : none;
+
     for (unsigned it = blockIdx.x; it < plan.total; it += gridDim.x) {
-        const Kv4Item m = kv4_item(a, plan, it);
-        const long long rows = (long long)m.fresh * a.H, row0 = (long long)m.tile * KA_ROWS;
-        const int nr = (int)min((long long)KA_ROWS, rows - row0);
         __syncthreads();
-        for (int i = tid; i < KA_ROWS * cols; i += KA_BLOCK) {
-            const int rr = i / cols, col = i % cols;
-            float v = 0.0f;
-            if (rr < nr) {
-                const long long g = row0 + rr, t = m.t0 + g / a.H;
-                const int h = (int)(g % a.H);
-                if (col < kv) v = a.q_abs[t * a.ld_q_abs + (long long)h * kv + col];
-                else if (col - kv < rope) v = a.q_pe[t * a.ld_q_pe + (long long)h * rope + col - kv];
+        ka_find<false>(a, plan, ROWS, it, &item);
+        __syncthreads();
+        const KaItem m = item;
+        const int rows = m.fresh * a.H, row0 = m.tile * ROWS, nr = min(ROWS, rows - row0);
+        const int first = m.context - m.fresh;  // the position of the request's first token
+        const int end = (int)min((long long)max(0, first + min(m.fresh, (row0 + nr - 1) / a.H + 1)), (long long)a.max_pages << shift);
+        const long long c0 = (long long)m.chunk * plan.chunk * KA_P;
+        const int s0 = (int)min(c0, (long long)end), s1 = (int)min(c0 + (long long)plan.chunk * KA_P, (long long)end);
+        const int nt = (s1 - s0 + KA_P - 1) / KA_P;
+        const int32_t *table = a.table + (size_t)m.r * a.max_pages;
+
+        // the lane's position of tile j: its page, and from the page its row
+        auto page_of = [&](int j) {
+            const int s = s0 + KA_P * j + 16 * pg + l16;
+            return s < s1 ? table[s >> shift] : -1;
+        };
+        auto fetch = [&](int j, int page) {
+            KaRaw x;
+            const int s = s0 + KA_P * j + 16 * pg + l16;
+            x.on = page >= 0 && page < a.c.n_pages;
+            x.q0 = x.q1 = (u32x4){0, 0, 0, 0};
+            x.q2 = x.w0 = x.w1 = x.w2 = 0;
+            if (x.on) {
+                const uint8_t *row = a.c.rows + (((size_t)page << shift) + (s & ((1 << shift) - 1))) * a.c.row_bytes;
+                const uint8_t *sb = row + 16 * nb + 8 * kh;
+                if (b0 < nb) x.q0 = *gbl((const u32x4 *)(row + 16 * b0));
+                if (b1 < nb) x.q1 = *gbl((const u32x4 *)(row + 16 * b1));
+                if (b2 < nb) x.q2 = *gbl((const unsigned *)(row + 16 * b2 + 4 * lg));
+                if (KA_HALF * kh < nb) {  // the row has 8 bytes from there on, and 12 in the first half
+                    const u32x2 v = *gbl((const u32x2 *)sb);
+                    x.w0 = v[0];
+                    x.w1 = v[1];
+                    if (kh == 0 || nb > 16) x.w2 = *gbl((const unsigned *)(sb + 8));
+                }
             }
-            q[rr][col] = v;
-        }
-        float acc[KA_ROWS][2];
+            return x;
+        };
+        int page = nt > 0 ? page_of(0) : -1;
+        KaRaw raw = fetch(0, page);
+        page = nt > 1 ? page_of(1) : -1;
+
+        // the queries: wave w stages rows RPW w .. as operand rows of halves, scaled by 2^-e
+        _Float16 *stage = val[0];
+        float lsum[RPW], ref[RPW];
+        int eq[RPW], last[RPW];
 #pragma unroll
-        for (int rr = 0; rr < KA_ROWS; rr++) acc[rr][0] = acc[rr][1] = 0.0f;
-        if (tid < KA_ROWS) {
-            ml[tid][0] = -INFINITY;
-            ml[tid][1] = 0.0f;
-        }
-        for (int s0 = m.s0; s0 < m.s1; s0 += P) {
-            __syncthreads();
-            for (int i = tid; i < P * lanes; i += KA_BLOCK) {
-                const int j = i / lanes, w = i % lanes, s = s0 + j;
-                float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-                bool ok = s < m.s1;
-                if (ok) {
-                    const int page = a.table[(size_t)m.r * a.max_pages + (s >> a.c.shift)];
-                    ok = page >= 0 && page < a.c.n_pages;
-                    if (ok) {
-                        const size_t slot = ((size_t)page << a.c.shift) + (s & ((1 << a.c.shift) - 1));
-                        const uint8_t *row = a.c.rows + slot * a.c.row_bytes;
-                        kv4_values(((const unsigned *)row)[w], row[16 * a.c.blocks + (w >> 2)], v);
-                    }
-                }
-                if (w == 0) on[j] = ok;
+        for (int i = 0; i < RPW; i++) {
+            const int r = RPW * w + i, g = row0 + min(r, nr - 1), t = g / a.H, h = g - t * a.H;
+            const float *qa = a.q_abs + (m.t0 + t) * a.ld_q_abs + (int64_t)h * kv, *qp = a.q_pe + (m.t0 + t) * a.ld_q_pe + (int64_t)h * rope;
+            float v[KV4_BLOCKS_MAX / 2];
+            float mx = 0.0f;
 #pragma unroll
-                for (int k = 0; k < 8; k++) kt[j][8 * w + k] = v[k];
+            for (int k = 0; k < KV4_BLOCKS_MAX / 2; k++) {
+                const int col = 64 * k + lane;
+                v[k] = col < kv ? qa[col] : col - kv < rope ? qp[col - kv] : 0.0f;
+                mx = fmaxf(mx, fabsf(v[k]));
             }
-            __syncthreads();
-            for (int i = tid; i < KA_ROWS * P; i += KA_BLOCK) {
-                const int rr = i / P, j = i % P;
-                float d = 0.0f;
-                for (int col = 0; col < cols; col++) d = fmaf(q[rr][col], kt[j][col], d);
-                const long long last = m.context - m.fresh + (row0 + rr) / a.H;
-                sc[rr][j] = rr < nr && on[j] && s0 + j <= last ? d * a.scale : -INFINITY;
+            mx = wave_max_dpp_f(mx);
+            const int e = mx < INFINITY ? spl_exp(mx) : 0;
+            _Float16 *hi = stage + (16 * (r >> 3) + 4 * ((r & 7) >> 1) + (r & 1)) * KA_QROW, *lo = hi + 2 * KA_QROW;
+#pragma unroll
+            for (int k = 0; k < KV4_BLOCKS_MAX / 2; k++) {
+                _Float16 x, y;
+                spl_split(ldexpf(v[k], -e), x, y);
+                hi[64 * k + lane] = x;
+                lo[64 * k + lane] = y;
             }
-            __syncthreads();
-            if (tid < KA_ROWS) {
-                float mx = ml[tid][0], l = ml[tid][1];
-                for (int j = 0; j < P; j++) mx = fmaxf(mx, sc[tid][j]);
-                const float ref = mx == -INFINITY ? 0.0f : mx, back = ml[tid][0] == -INFINITY ? 0.0f : expf(ml[tid][0] - ref);
-                l *= back;
-                for (int j = 0; j < P; j++) {
-                    const float x = sc[tid][j], e = x == -INFINITY ? 0.0f : expf(x - ref);
-                    sc[tid][j] = e;
-                    l += e;
-                }
-                ml[tid][0] = mx;
-                ml[tid][1] = l;
-                cr[tid] = back;
-            }
-            __syncthreads();
-            for (int rr = 0; rr < KA_ROWS; rr++) {
-                acc[rr][0] *= cr[rr];
-                acc[rr][1] *= cr[rr];
-            }
-            for (int j = 0; j < P; j++) {
-                const float v0 = kt[j][tid], v1 = kt[j][tid + KA_BLOCK];
-                for (int rr = 0; rr < KA_ROWS; rr++) {
-                    const float e = sc[rr][j];
-                    if (e != 0.0f) {  // a masked position's value may be NaN
-                        acc[rr][0] = fmaf(e, v0, acc[rr][0]);
-                        acc[rr][1] = fmaf(e, v1, acc[rr][1]);
-                    }
-                }
-            }
+            eq[i] = e;
+            last[i] = min(first + t, s1 - 1);
+            lsum[i] = 0.0f;
+            ref[i] = -INFINITY;
         }
         __syncthreads();
-        for (int rr = 0; rr < nr; rr++) {
-            const float l = ml[rr][1];
-            float *dst;
-            float f = 1.0f;
-            if (m.k > 1) {
-                dst = a.part + ((size_t)m.part * KA_ROWS + rr) * kv;
-                if (tid < 2) a.part_ml[((size_t)m.part * KA_ROWS + rr) * 2 + tid] = ml[rr][tid];
-            } else {
-                const long long g = row0 + rr, t = m.t0 + g / a.H;
-                dst = a.out + t * a.ld_out + (g % a.H) * kv;
-                f = l == 0.0f ? 0.0f : 1.0f / l;
+        a16_h8 q[KA_HALF][MT];  // steps 0..3: eighths of blocks j; 4..7: of blocks 4 + j; 8: block 8
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            const _Float16 *src = stage + (16 * mt + l16) * KA_QROW;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                q[k][mt] = *(const a16_h8 *)(src + 32 * b0 + 8 * k);
+                q[4 + k][mt] = *(const a16_h8 *)(src + 32 * b1 + 8 * k);
             }
-            if (tid < kv) dst[tid] = f == 0.0f ? 0.0f : acc[rr][0] * f;
-            if (tid + KA_BLOCK < kv) dst[tid + KA_BLOCK] = f == 0.0f ? 0.0f : acc[rr][1] * f;
+            q[8][mt] = *(const a16_h8 *)(src + 32 * b2 + 8 * lg);
+        }
+        aq_f4 acc[4][MT];
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) acc[c][mt] = (aq_f4){0.0f, 0.0f, 0.0f, 0.0f};
+        __syncthreads();  // the staged queries are read; values may come
+
+        // tile j's scores (this half's part) from `raw`, its values to shared memory
+        auto scores = [&](int j) {
+            unsigned e0 = __builtin_amdgcn_perm(raw.w1, raw.w0, sel0), e1 = __builtin_amdgcn_perm(raw.w2, raw.w1, sel1),
+                     e2 = __builtin_amdgcn_perm(0u, raw.w2, sel2);
+            const bool bad = max(max(e0, e1), e2) == KV4_BYTE_NAN;
+            unsigned long long spoilt = __ballot(bad);
+            if (spoilt) {  // such a block's values count as zeros, and its position's scores as NaN
+                if (e0 == KV4_BYTE_NAN) e0 = 0;
+                if (e1 == KV4_BYTE_NAN) e1 = 0;
+                if (e2 == KV4_BYTE_NAN) e2 = 0;
+                spoilt |= spoilt >> 32;
+                spoilt |= spoilt >> 16;
+            }
+            const float f0 = __uint_as_float(e0 << 23), f1 = __uint_as_float(e1 << 23), f2 = __uint_as_float(e2 << 23);
+            const int p = 16 * pg + l16;
+            _Float16 *dst = val[j & 1] + p * KA_VROW;
+            const int flip = p & 8;  // rows r and r + 8 have the halves of 16 columns the other way round, in other banks
+            aq_f4 d[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) d[mt] = (aq_f4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < KA_HALF; k++) {
+                const a16_h8 x = k < 4 ? ka_halves(raw.q0[k & 3], f0) : k < 8 ? ka_halves(raw.q1[k & 3], f1) : ka_halves(raw.q2, f2);
+                const int col = k < 4 ? 32 * b0 + 8 * k : k < 8 ? 32 * b1 + 8 * (k - 4) : 32 * b2 + 8 * lg;
+                if (col < kv) *(a16_h8 *)(dst + (col ^ flip)) = x;
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) d[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[k][mt], x, d[mt], 0, 0, 0);
+            }
+            const float nan = __uint_as_float(0x7fc00000u);
+            const bool mark = spoilt >> l16 & 1;
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                float2 s = make_float2(d[mt][0] + d[mt][2], d[mt][1] + d[mt][3]);
+                if (spoilt && mark) s = make_float2(nan, nan);
+                if (!raw.on) s = make_float2(-INFINITY, -INFINITY);
+                *(float2 *)&sc[kh][p][8 * mt + 2 * lg] = s;
+            }
+        };
+        // tile j's exponentials from its scores
+        auto softmax = [&](int j) {
+            const int s = s0 + KA_P * j + lane;
+            const int at = 32 * (lane >> 5) + 8 * ((lane & 15) >> 2) + 4 * ((lane & 31) >> 4) + (lane & 3);  // the position's operand slot
+            int any = 0;
+#pragma unroll
+            for (int i = 0; i < RPW; i++) {
+                const int r = RPW * w + i;
+                const float x = sc[0][lane][r] + sc[1][lane][r];
+                const float y = x == -INFINITY || s > last[i] ? -INFINITY : __fmul_rn(ldexpf(x, eq[i]), a.scale);
+                const float mx = wave_max_dpp_f(y) * L;
+                float f = 1.0f;
+                if (mx > ref[i] + KA_SLACK) {  // (ref is -inf before the first position)
+                    f = __builtin_amdgcn_exp2f(ref[i] - mx);
+                    ref[i] = mx;
+                    any = 1;
+                }
+                const float e = __builtin_amdgcn_exp2f(fmaf(y, L, ref[i] == -INFINITY ? 0.0f : -ref[i]));
+                lsum[i] = fmaf(lsum[i], f, e);
+                _Float16 hi, lo;
+                spl_split(ldexpf(e, KA_UP), hi, lo);
+                _Float16 *dst = &pr[16 * (r >> 3) + 4 * ((r & 7) >> 1) + (r & 1)][at];
+                dst[0] = hi;
+                dst[2 * KA_PROW] = lo;
+                if (lane == 0) cr[r] = f;
+            }
+            if (lane == 0) moved[w] = any;
+        };
+        // tile j's values weighted
+        auto values = [&](int j) {
+            int any = 0;
+#pragma unroll
+            for (int i = 0; i < KA_WAVES; i++) any |= moved[i];
+            if (__builtin_amdgcn_readfirstlane(any)) {
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) {
+                    const float2 f = *(const float2 *)&cr[8 * mt + 2 * lg];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) acc[c][mt] *= (aq_f4){f.x, f.y, f.x, f.y};
+                }
+            }
+            const _Float16 *src = val[j & 1] + (4 * lg + (l16 >> 2)) * KA_VROW + ((64 * w + 4 * (l16 & 3)) ^ (lg & 2 ? 8 : 0));
+#pragma unroll
+            for (int ks = 0; ks < KA_P / 32; ks++) {
+                a16_h8 p[MT];
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) p[mt] = *(const a16_h8 *)&pr[16 * mt + l16][32 * ks + 8 * lg];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const a16_h4 x = a16_tr(src + 32 * ks * KA_VROW + 16 * c), y = a16_tr(src + (32 * ks + 16) * KA_VROW + 16 * c);
+                    const a16_h8 v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) acc[c][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[mt], v, acc[c][mt], 0, 0, 0);
+                }
+            }
+        };
+        const bool mine = 64 * w < kv;  // the wave has columns
+        if (nt > 0) {
+            for (int j = 0; j <= nt; j++) {
+                if (j < nt) {
+                    KaRaw next = raw;
+                    if (j + 1 < nt) {
+                        next = fetch(j + 1, page);
+                        page = j + 2 < nt ? page_of(j + 2) : -1;
+                    }
+                    scores(j);
+                    raw = next;
+                }
+                if (j > 0 && mine) values(j - 1);
+                block_barrier();
+                if (j < nt) {
+                    softmax(j);
+                    block_barrier();
+                }
+            }
+        }
+        // the rows' sums to every wave, and the results
+#pragma unroll
+        for (int i = 0; i < RPW; i++) {
+            float l = row_sum_dpp_f(lsum[i]);
+            l = (readlane_f(l, 0) + readlane_f(l, 16)) + (readlane_f(l, 32) + readlane_f(l, 48));
+            if (lane == 0) {
+                rl[RPW * w + i] = l;
+                rm[RPW * w + i] = ref[i];
+            }
+        }
+        __syncthreads();
+        if (m.k > 1 && tid < nr) {
+            float *ml = a.part_ml + ((size_t)m.part * KA_ROWS + tid) * 2;
+            ml[0] = rm[tid];
+            ml[1] = rl[tid];
+        }
+        if (mine) {
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int r = 8 * mt + 2 * lg + i;
+                    if (r >= nr) continue;
+                    float *dst;
+                    float f = 1.0f / (1 << KA_UP);
+                    if (m.k > 1) {
+                        dst = a.part + ((size_t)m.part * KA_ROWS + r) * kv;
+                    } else {
+                        const int g = row0 + r, t = g / a.H;
+                        dst = a.out + (m.t0 + t) * a.ld_out + (int64_t)(g - t * a.H) * kv;
+                        f = rl[r] == 0.0f ? 0.0f : f / rl[r];
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const int col = 64 * w + 16 * c + l16;
+                        if (col < kv) dst[col] = (acc[c][mt][i] + acc[c][mt][i + 2]) * f;
+                    }
+                }
         }
     }
 }
 
 // The cut tiles' partial results joined, a block a query row: out = sum_c w_c part_c / sum_c w_c l_c
-// with w_c = exp(m_c - m).
-__global__ __launch_bounds__(KA_BLOCK) void k_kv4_merge(Kv4Attn a) {
-    __shared__ Kv4Plan plan;
-    __shared__ float wgt[KA_MAX_PARTS];
-    __shared__ float red[KA_BLOCK / 64];
+// with w_c = 2^(ref_c - max ref). Threads have four columns each; the groups that cover a row share
+// its chunks.
+__global__ __launch_bounds__(KA_BLOCK) void k_kv4_merge(Kv4Attn a, int rows) {
+    __shared__ KaShared sh;
+    __shared__ KaItem item;
+    __shared__ float wgt[KA_ITEMS];
+    __shared__ float red[KA_WAVES];
+    __shared__ __align__(16) float4 sum[KA_BLOCK];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, kv = a.c.kv;
-    kv4_plan(a, plan);
-    unsigned i = 0;
-    for (unsigned unit = blockIdx.x;; unit += gridDim.x) {
-        // the unit-th row slot of the cut tiles
-        const unsigned ti = unit / KA_ROWS, rr = unit % KA_ROWS;
-        // walk the items to the ti-th cut tile
-        unsigned seen = 0;
-        bool found = false;
-        for (int r = 0; r < a.R; r++) {
-            const unsigned n = plan.items[r] - (r > 0 ? plan.items[r - 1] : 0u);
-            const unsigned k = max(1u, (ka_units(a, r) + plan.chunk - 1) / plan.chunk);
-            if (k < 2 || n == 0) continue;
-            if (ti < seen + n / k) {
-                i = (r > 0 ? plan.items[r - 1] : 0u) + (ti - seen) * k;
-                found = true;
-                break;
-            }
-            seen += n / k;
+    const KaPlan plan = ka_plan(a, rows, sh);
+    const int cols = kv / 4, groups = KA_BLOCK / cols, grp = tid / cols, col = tid - grp * cols;
+    for (unsigned unit = blockIdx.x; unit < plan.total_cuts * rows; unit += gridDim.x) {
+        const unsigned ti = unit / rows;
+        const int rr = (int)(unit - ti * rows);
+        __syncthreads();
+        ka_find<true>(a, plan, rows, ti, &item);
+        __syncthreads();
+        const KaItem m = item;
+        const int g = m.tile * rows + rr;
+        if (g >= m.fresh * a.H) continue;
+        const float *ml = a.part_ml + ((size_t)m.part * KA_ROWS + rr) * 2;
+        float pm = -INFINITY, pl = 0.0f;
+        if (tid < m.k) {
+            pm = ml[(size_t)tid * KA_ROWS * 2];
+            pl = ml[(size_t)tid * KA_ROWS * 2 + 1];
         }
-        if (!found) return;
-        const Kv4Item m = kv4_item(a, plan, i);
-        const long long g = (long long)m.tile * KA_ROWS + rr;
-        if (g >= (long long)m.fresh * a.H) continue;
-        const float *pml = a.part_ml + ((size_t)m.part * KA_ROWS + rr) * 2;
-        float mx = -INFINITY;
-        for (int c = tid; c < m.k; c += KA_BLOCK) mx = fmaxf(mx, pml[(size_t)c * KA_ROWS * 2]);
-        mx = wave_max_dpp_f(mx);
+        const float wm = wave_max_dpp_f(pm);
+        if (lane == 0) red[w] = wm;
         __syncthreads();
-        if (lane == 0) red[w] = mx;
+        float mx = red[0];
+#pragma unroll
+        for (int i = 1; i < KA_WAVES; i++) mx = fmaxf(mx, red[i]);
         __syncthreads();
-        mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        __syncthreads();
-        float l = 0.0f;
-        for (int c = tid; c < m.k; c += KA_BLOCK) {
-            const float pm = pml[(size_t)c * KA_ROWS * 2], pl = pml[(size_t)c * KA_ROWS * 2 + 1];
-            const float e = pl == 0.0f ? 0.0f : expf(pm - mx);
-            wgt[c] = e;
-            l = fmaf(pl, e, l);
-        }
-        for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d);
+        const float e = pl == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(pm - mx);
+        if (tid < m.k) wgt[tid] = e;
+        float l = row_sum_dpp_f(e * pl);
+        l = (readlane_f(l, 0) + readlane_f(l, 16)) + (readlane_f(l, 32) + readlane_f(l, 48));
         if (lane == 0) red[w] = l;
         __syncthreads();
-        l = (red[0] + red[1]) + (red[2] + red[3]);
-        float *dst = a.out + (m.t0 + g / a.H) * a.ld_out + (g % a.H) * kv;
-        for (int col = tid; col < kv; col += KA_BLOCK) {
-            const float *pc = a.part + ((size_t)m.part * KA_ROWS + rr) * kv + col;
-            float s = 0.0f;
-            for (int c = 0; c < m.k; c++)
-                if (wgt[c] != 0.0f) s = fmaf(wgt[c], pc[(size_t)c * KA_ROWS * kv], s);
-            dst[col] = l == 0.0f ? 0.0f : s / l;
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < KA_WAVES; i++) l += red[i];
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (grp < groups) {
+            const float *pc = a.part + ((size_t)m.part * KA_ROWS + rr) * kv + 4 * col;
+#pragma unroll 4
+            for (int c = grp; c < m.k; c += groups) {
+                const float4 v = *(const float4 *)(pc + (size_t)c * KA_ROWS * kv);
+                const float x = wgt[c];
+                s.x = fmaf(x, v.x, s.x);
+                s.y = fmaf(x, v.y, s.y);
+                s.z = fmaf(x, v.z, s.z);
+                s.w = fmaf(x, v.w, s.w);
+            }
+        }
+        sum[tid] = s;
+        __syncthreads();
+        if (tid < cols) {
+            for (int k = 1; k < groups; k++) {
+                const float4 v = sum[tid + k * cols];
+                s.x += v.x;
+                s.y += v.y;
+                s.z += v.z;
+                s.w += v.w;
+            }
+            const int t = g / a.H;
+            float *dst = a.out + (m.t0 + t) * a.ld_out + (int64_t)(g - t * a.H) * kv + 4 * tid;
+            const float f = l == 0.0f ? 0.0f : 1.0f / l;
+            dst[0] = s.x * f;
+            dst[1] = s.y * f;
+            dst[2] = s.z * f;
+            dst[3] = s.w * f;
         }
     }
+}
+
+// Operand tiles a row tile for rows of a request's step, by the cost of the tiles it takes: each
+// converts the cache's codes once (about one operand tile's products) and multiplies MT operand tiles.
+static inline int ka_operand_tiles(long long rows) {
+    int best = 1;
+    long long least = 1ll << 62;
+    for (int mt = 1; mt <= KA_ROWS / 8; mt++) {
+        const long long cost = (rows + 8 * mt - 1) / (8 * mt) * (1 + mt);
+        if (cost < least) {
+            least = cost;
+            best = mt;
+        }
+    }
+    return best;
 }

@@ -183,8 +183,12 @@ extern "C" int gmoe_kv4_attend(int device, const gmoe_kv4 *c, const gmoe_batch *
     OnDevice on(device);
     if (on.err != hipSuccess) return failed("gmoe_kv4_attend: the device", on.err);
     hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(k_kv4_attend, dim3(KA_ITEMS), dim3(KA_BLOCK), 0, st, a);
-    hipLaunchKernelGGL(k_kv4_merge, dim3(KA_ITEMS), dim3(KA_BLOCK), 0, st, a);
+    // the host knows no request's tokens: it takes them all alike
+    const int mt = ka_operand_tiles((long long)a.H * ((b->max_tokens + a.R - 1) / a.R));
+    if (mt == 1) hipLaunchKernelGGL(k_kv4_attend<1>, dim3(KA_GRID), dim3(KA_BLOCK), 0, st, a);
+    else if (mt == 2) hipLaunchKernelGGL(k_kv4_attend<2>, dim3(KA_GRID), dim3(KA_BLOCK), 0, st, a);
+    else hipLaunchKernelGGL(k_kv4_attend<3>, dim3(KA_GRID), dim3(KA_BLOCK), 0, st, a);
+    hipLaunchKernelGGL(k_kv4_merge, dim3(KA_GRID), dim3(KA_BLOCK), 0, st, a, 8 * mt);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? GMOE_OK : failed("gmoe_kv4_attend", e);
 }
