@@ -60,7 +60,7 @@ struct Kv4Attn {
     int64_t ld_q_abs, ld_q_pe, ld_out;
     float *out;
     float *part;     // [KA_MAX_PARTS][KA_ROWS][kv]
-    float *part_ml;  // [KA_MAX_PARTS][KA_ROWS][2]: a chunk's reference (of base 2) and its sum of exponentials
+    float *part_ml;  // [KA_MAX_PARTS][KA_ROWS][2]: a chunk's reference (of base 2, to a constant) and its sum of exponentials
 };
 
 // ---- the split of a launch -------------------------------------------------------------------
@@ -167,9 +167,18 @@ __device__ static inline a16_h8 ka_halves(unsigned codes, float scale) {
 struct KaRaw {
     u32x4 q0, q1;  // blocks j and 4 + j of the half (j = lane / 16)
     unsigned q2;   // the lane's eighth of block 8
-    unsigned w0, w1, w2;  // the half's scale bytes, from byte 0 (first half) or 1 on
-    bool on;
+    u32x2 w0;      // the half's scale bytes, from byte 0 (first half) or 1 on: eight,
+    unsigned w1;   // and the next four
+    unsigned on;   // all ones, or 0 where there is no such position
 };
+
+// The thread's index as the compiler cannot know it, so that addresses made from it are not kept in
+// registers (or out of them) across the loop over items.
+__device__ static inline int ka_tid() {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
 
 template <int MT>
 __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
@@ -178,19 +187,14 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
     __shared__ __align__(16) _Float16 val[2][KA_P * KA_VROW];
     __shared__ __align__(16) float sc[2][KA_P][KA_SROW];
     __shared__ __align__(16) _Float16 pr[OPS][KA_PROW];
-    __shared__ float cr[ROWS], rl[ROWS], rm[ROWS];
-    __shared__ int moved[KA_WAVES];
+    __shared__ __align__(8) float cr[ROWS], rl[ROWS], rm[ROWS];
+    __shared__ __align__(8) unsigned char moved[KA_WAVES];
     __shared__ KaShared sh;
     __shared__ KaItem item;
-    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), kh = w >> 2, pg = w & 3;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kh = w >> 2, pg = w & 3;
     const int kv = a.c.kv, rope = a.c.rope, nb = a.c.blocks, shift = a.c.shift;
     const KaPlan plan = ka_plan(a, ROWS, sh);
-    const float L = 1.44269504f;
-    // the lane's blocks of its half, and where their scales lie in the half's bytes
-    const int b0 = KA_HALF * kh + lg, b1 = b0 + 4, b2 = KA_HALF * kh + 8;
-    const unsigned none = 0x0c0c0c0cu, sel0 = b0 < nb ? 0x0c0c0c00u + kh + lg : none, sel1 = b1 < nb ? 0x0c0c0c00u + kh + lg : none,
-                   sel2 = b2 < nb ? 0x0c0c0c00u + kh : none;
+    const float scale = __fmul_rn(a.scale, 1.44269504f);  // scores of base 2
 
     for (unsigned it = blockIdx.x; it < plan.total; it += gridDim.x) {
         __syncthreads();
@@ -205,40 +209,43 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
         const int nt = (s1 - s0 + KA_P - 1) / KA_P;
         const int32_t *table = a.table + (size_t)m.r * a.max_pages;
 
-        // the lane's position of tile j: its page, and from the page its row
-        auto page_of = [&](int j) {
+        const int tid = ka_tid(), lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
+        // The lane's blocks of its half, and which of the half's bytes are their scales. A block past the
+        // row's last reads codes of another at scale 0.
+        const int b0 = KA_HALF * kh + lg, b1 = b0 + 4, b2 = KA_HALF * kh + 8;
+        const unsigned none = 0x0c0c0c0cu, sel0 = b0 < nb ? 0x0c0c0c00u + kh + lg : none, sel1 = b1 < nb ? 0x0c0c0c00u + kh + lg : none,
+                       sel2 = b2 < nb ? 0x0c0c0c00u + kh : none;
+        const int at0 = b0 < nb ? 16 * b0 : 0, at1 = b1 < nb ? 16 * b1 : 0, at2 = b2 < nb ? 16 * b2 + 4 * lg : 0;
+        // (a row ends 16 bytes past its codes, 32 where it has over 16 blocks)
+        const int ats = 16 * nb + (KA_HALF * kh < nb ? 8 * kh : 0), atw = 16 * nb + (kh == 0 ? 8 : nb > 16 ? 16 : 0);
+        const bool v0 = 32 * b0 < kv, v1 = 32 * b1 < kv, v2 = 32 * b2 < kv;  // blocks of the entry, not of the rope part
+        // the lane's position of tile j: its page, as the table has it (nothing looks at it before fetch(),
+        // so that nothing waits for it), and from the page its row
+        auto page_of = [&](int j) { return *gbl(table + (min(s0 + KA_P * j + 16 * pg + l16, s1 - 1) >> shift)); };
+        auto fetch = [&](KaRaw &x, int j, int page) {
             const int s = s0 + KA_P * j + 16 * pg + l16;
-            return s < s1 ? table[s >> shift] : -1;
+            x.on = s < s1 && page >= 0 && page < a.c.n_pages ? ~0u : 0u;
+            const unsigned slot = x.on & (((unsigned)page << shift) + (s & ((1 << shift) - 1)));
+            const uint8_t *row = a.c.rows + (size_t)slot * (unsigned)a.c.row_bytes;
+            x.q0 = *gbl((const u32x4 *)(row + at0));
+            x.q1 = *gbl((const u32x4 *)(row + at1));
+            x.q2 = *gbl((const unsigned *)(row + at2));
+            x.w0 = *gbl((const u32x2 *)(row + ats));
+            x.w1 = *gbl((const unsigned *)(row + atw));
         };
-        auto fetch = [&](int j, int page) {
-            KaRaw x;
-            const int s = s0 + KA_P * j + 16 * pg + l16;
-            x.on = page >= 0 && page < a.c.n_pages;
-            x.q0 = x.q1 = (u32x4){0, 0, 0, 0};
-            x.q2 = x.w0 = x.w1 = x.w2 = 0;
-            if (x.on) {
-                const uint8_t *row = a.c.rows + (((size_t)page << shift) + (s & ((1 << shift) - 1))) * a.c.row_bytes;
-                const uint8_t *sb = row + 16 * nb + 8 * kh;
-                if (b0 < nb) x.q0 = *gbl((const u32x4 *)(row + 16 * b0));
-                if (b1 < nb) x.q1 = *gbl((const u32x4 *)(row + 16 * b1));
-                if (b2 < nb) x.q2 = *gbl((const unsigned *)(row + 16 * b2 + 4 * lg));
-                if (KA_HALF * kh < nb) {  // the row has 8 bytes from there on, and 12 in the first half
-                    const u32x2 v = *gbl((const u32x2 *)sb);
-                    x.w0 = v[0];
-                    x.w1 = v[1];
-                    if (kh == 0 || nb > 16) x.w2 = *gbl((const unsigned *)(sb + 8));
-                }
-            }
-            return x;
-        };
-        int page = nt > 0 ? page_of(0) : -1;
-        KaRaw raw = fetch(0, page);
-        page = nt > 1 ? page_of(1) : -1;
+        int page = -1;
+        KaRaw raw;
+        if (nt > 0) {
+            fetch(raw, 0, page_of(0));
+            if (nt > 1) page = page_of(1);
+        }
 
         // the queries: wave w stages rows RPW w .. as operand rows of halves, scaled by 2^-e
         _Float16 *stage = val[0];
-        float lsum[RPW], ref[RPW];
+        const int plane = ka_tid() & 63;
+        float lsum[RPW], top[RPW];  // a row's sum, and its reference + KA_SLACK (of base 2)
         int eq[RPW], last[RPW];
+        bool on[RPW];
 #pragma unroll
         for (int i = 0; i < RPW; i++) {
             const int r = RPW * w + i, g = row0 + min(r, nr - 1), t = g / a.H, h = g - t * a.H;
@@ -247,7 +254,7 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
             float mx = 0.0f;
 #pragma unroll
             for (int k = 0; k < KV4_BLOCKS_MAX / 2; k++) {
-                const int col = 64 * k + lane;
+                const int col = 64 * k + plane;
                 v[k] = col < kv ? qa[col] : col - kv < rope ? qp[col - kv] : 0.0f;
                 mx = fmaxf(mx, fabsf(v[k]));
             }
@@ -258,13 +265,13 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
             for (int k = 0; k < KV4_BLOCKS_MAX / 2; k++) {
                 _Float16 x, y;
                 spl_split(ldexpf(v[k], -e), x, y);
-                hi[64 * k + lane] = x;
-                lo[64 * k + lane] = y;
+                hi[64 * k + plane] = x;
+                lo[64 * k + plane] = y;
             }
             eq[i] = e;
             last[i] = min(first + t, s1 - 1);
             lsum[i] = 0.0f;
-            ref[i] = -INFINITY;
+            top[i] = -INFINITY;
         }
         __syncthreads();
         a16_h8 q[KA_HALF][MT];  // steps 0..3: eighths of blocks j; 4..7: of blocks 4 + j; 8: block 8
@@ -287,10 +294,9 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
 
         // tile j's scores (this half's part) from `raw`, its values to shared memory
         auto scores = [&](int j) {
-            unsigned e0 = __builtin_amdgcn_perm(raw.w1, raw.w0, sel0), e1 = __builtin_amdgcn_perm(raw.w2, raw.w1, sel1),
-                     e2 = __builtin_amdgcn_perm(0u, raw.w2, sel2);
-            const bool bad = max(max(e0, e1), e2) == KV4_BYTE_NAN;
-            unsigned long long spoilt = __ballot(bad);
+            unsigned e0 = __builtin_amdgcn_perm(raw.w0[1], raw.w0[0], sel0) & raw.on, e1 = __builtin_amdgcn_perm(raw.w1, raw.w0[1], sel1) & raw.on,
+                     e2 = __builtin_amdgcn_perm(0u, raw.w1, sel2) & raw.on;
+            unsigned long long spoilt = __ballot(max(max(e0, e1), e2) == KV4_BYTE_NAN);
             if (spoilt) {  // such a block's values count as zeros, and its position's scores as NaN
                 if (e0 == KV4_BYTE_NAN) e0 = 0;
                 if (e1 == KV4_BYTE_NAN) e1 = 0;
@@ -300,63 +306,91 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
             }
             const float f0 = __uint_as_float(e0 << 23), f1 = __uint_as_float(e1 << 23), f2 = __uint_as_float(e2 << 23);
             const int p = 16 * pg + l16;
+            // rows r and r + 8 have the halves of 16 columns the other way round, in other banks
             _Float16 *dst = val[j & 1] + p * KA_VROW;
-            const int flip = p & 8;  // rows r and r + 8 have the halves of 16 columns the other way round, in other banks
+            const int flip = p & 8;
             aq_f4 d[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) d[mt] = (aq_f4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int k = 0; k < KA_HALF; k++) {
-                const a16_h8 x = k < 4 ? ka_halves(raw.q0[k & 3], f0) : k < 8 ? ka_halves(raw.q1[k & 3], f1) : ka_halves(raw.q2, f2);
-                const int col = k < 4 ? 32 * b0 + 8 * k : k < 8 ? 32 * b1 + 8 * (k - 4) : 32 * b2 + 8 * lg;
-                if (col < kv) *(a16_h8 *)(dst + (col ^ flip)) = x;
+            for (int g = 0; g < 2; g++) {
+                a16_h8 x[4];
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++) d[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[k][mt], x, d[mt], 0, 0, 0);
-            }
-            const float nan = __uint_as_float(0x7fc00000u);
-            const bool mark = spoilt >> l16 & 1;
+                for (int k = 0; k < 4; k++) x[k] = ka_halves(g ? raw.q1[k] : raw.q0[k], g ? f1 : f0);
+                if (g ? v1 : v0) {
+                    _Float16 *at = dst + 32 * (g ? b1 : b0);
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                float2 s = make_float2(d[mt][0] + d[mt][2], d[mt][1] + d[mt][3]);
-                if (spoilt && mark) s = make_float2(nan, nan);
-                if (!raw.on) s = make_float2(-INFINITY, -INFINITY);
-                *(float2 *)&sc[kh][p][8 * mt + 2 * lg] = s;
+                    for (int k = 0; k < 4; k++) *(a16_h8 *)(at + ((8 * k) ^ flip)) = x[k];
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) d[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[4 * g + k][mt], x[k], d[mt], 0, 0, 0);
             }
+            const a16_h8 x = ka_halves(raw.q2, f2);
+            if (v2) *(a16_h8 *)(dst + 32 * b2 + ((8 * lg) ^ flip)) = x;
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) d[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[8][mt], x, d[mt], 0, 0, 0);
+            float2 t[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) t[mt] = make_float2(d[mt][0] + d[mt][2], d[mt][1] + d[mt][3]);
+            if (spoilt || !__all(raw.on)) {
+                const float odd = !raw.on ? -INFINITY : __uint_as_float(0x7fc00000u);
+                if (!raw.on || (spoilt >> l16 & 1))
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) t[mt] = make_float2(odd, odd);
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) *(float2 *)&sc[kh][p][8 * mt + 2 * lg] = t[mt];
         };
         // tile j's exponentials from its scores
+        const int slot_at = 32 * (lane >> 5) + 8 * ((lane & 15) >> 2) + 4 * ((lane & 31) >> 4) + (lane & 3);  // a position's operand slot
+        _Float16 *const pdst = &pr[0][slot_at];
         auto softmax = [&](int j) {
             const int s = s0 + KA_P * j + lane;
-            const int at = 32 * (lane >> 5) + 8 * ((lane & 15) >> 2) + 4 * ((lane & 31) >> 4) + (lane & 3);  // the position's operand slot
-            int any = 0;
+            float t[RPW];
+            bool up[RPW], any = false;
+#pragma unroll
+            for (int i = 0; i < RPW; i++) {
+                const float x = sc[0][lane][RPW * w + i] + sc[1][lane][RPW * w + i];
+                t[i] = ldexpf(x, eq[i]);
+                on[i] = s <= last[i] && x != -INFINITY;
+                up[i] = on[i] && t[i] * scale > top[i];
+                any |= up[i];
+            }
+            const bool move = __any(any);
+            float mine = 1.0f;  // lane i: row i's factor
+            if (move) {
+#pragma unroll
+                for (int i = 0; i < RPW; i++) {
+                    const float mx = wave_max_dpp_f(on[i] ? t[i] * scale : -INFINITY);
+                    float f = 1.0f;
+                    if (mx > top[i]) {
+                        f = __builtin_amdgcn_exp2f((top[i] - KA_SLACK) - mx);  // 0 before the first position
+                        top[i] = mx + KA_SLACK;
+                    }
+                    lsum[i] *= f;
+                    mine = lane == i ? f : mine;
+                }
+            }
+            if (lane < RPW) cr[RPW * w + lane] = mine;
+            if (lane == 0) moved[w] = move;
 #pragma unroll
             for (int i = 0; i < RPW; i++) {
                 const int r = RPW * w + i;
-                const float x = sc[0][lane][r] + sc[1][lane][r];
-                const float y = x == -INFINITY || s > last[i] ? -INFINITY : __fmul_rn(ldexpf(x, eq[i]), a.scale);
-                const float mx = wave_max_dpp_f(y) * L;
-                float f = 1.0f;
-                if (mx > ref[i] + KA_SLACK) {  // (ref is -inf before the first position)
-                    f = __builtin_amdgcn_exp2f(ref[i] - mx);
-                    ref[i] = mx;
-                    any = 1;
-                }
-                const float e = __builtin_amdgcn_exp2f(fmaf(y, L, ref[i] == -INFINITY ? 0.0f : -ref[i]));
-                lsum[i] = fmaf(lsum[i], f, e);
-                _Float16 hi, lo;
-                spl_split(ldexpf(e, KA_UP), hi, lo);
-                _Float16 *dst = &pr[16 * (r >> 3) + 4 * ((r & 7) >> 1) + (r & 1)][at];
+                const float ref = top[i] - (KA_SLACK + KA_UP);
+                const float e = on[i] ? __builtin_amdgcn_exp2f(fmaf(t[i], scale, -ref)) : 0.0f;
+                lsum[i] += e;
+                _Float16 *dst = pdst + (16 * (r >> 3) + 4 * ((r & 7) >> 1) + (r & 1)) * KA_PROW;
+                const _Float16 hi = (_Float16)e;
                 dst[0] = hi;
-                dst[2 * KA_PROW] = lo;
-                if (lane == 0) cr[r] = f;
+                dst[2 * KA_PROW] = (_Float16)fmaf((float)hi, -1.0f, e);
             }
-            if (lane == 0) moved[w] = any;
         };
         // tile j's values weighted
         auto values = [&](int j) {
-            int any = 0;
-#pragma unroll
-            for (int i = 0; i < KA_WAVES; i++) any |= moved[i];
-            if (__builtin_amdgcn_readfirstlane(any)) {
+            const u32x2 mv = *(const u32x2 *)moved;
+            if (__builtin_amdgcn_readfirstlane(mv[0] | mv[1])) {
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++) {
                     const float2 f = *(const float2 *)&cr[8 * mt + 2 * lg];
@@ -383,13 +417,11 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
         if (nt > 0) {
             for (int j = 0; j <= nt; j++) {
                 if (j < nt) {
-                    KaRaw next = raw;
-                    if (j + 1 < nt) {
-                        next = fetch(j + 1, page);
-                        page = j + 2 < nt ? page_of(j + 2) : -1;
-                    }
                     scores(j);
-                    raw = next;
+                    if (j + 1 < nt) {
+                        fetch(raw, j + 1, page);
+                        if (j + 2 < nt) page = page_of(j + 2);
+                    }
                 }
                 if (j > 0 && mine) values(j - 1);
                 block_barrier();
@@ -400,40 +432,41 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
             }
         }
         // the rows' sums to every wave, and the results
+        const int etid = ka_tid(), elane = etid & 63;
 #pragma unroll
         for (int i = 0; i < RPW; i++) {
             float l = row_sum_dpp_f(lsum[i]);
             l = (readlane_f(l, 0) + readlane_f(l, 16)) + (readlane_f(l, 32) + readlane_f(l, 48));
-            if (lane == 0) {
+            if (elane == 0) {
                 rl[RPW * w + i] = l;
-                rm[RPW * w + i] = ref[i];
+                rm[RPW * w + i] = top[i];
             }
         }
         __syncthreads();
-        if (m.k > 1 && tid < nr) {
-            float *ml = a.part_ml + ((size_t)m.part * KA_ROWS + tid) * 2;
-            ml[0] = rm[tid];
-            ml[1] = rl[tid];
+        if (m.k > 1 && etid < nr) {
+            float *ml = a.part_ml + ((size_t)m.part * KA_ROWS + etid) * 2;
+            ml[0] = rm[etid];
+            ml[1] = rl[etid];
         }
         if (mine) {
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const int r = 8 * mt + 2 * lg + i;
+                    const int r = 8 * mt + 2 * (elane >> 4) + i;
                     if (r >= nr) continue;
                     float *dst;
-                    float f = 1.0f / (1 << KA_UP);
+                    float f = 1.0f;
                     if (m.k > 1) {
                         dst = a.part + ((size_t)m.part * KA_ROWS + r) * kv;
                     } else {
                         const int g = row0 + r, t = g / a.H;
                         dst = a.out + (m.t0 + t) * a.ld_out + (int64_t)(g - t * a.H) * kv;
-                        f = rl[r] == 0.0f ? 0.0f : f / rl[r];
+                        f = rl[r] == 0.0f ? 0.0f : 1.0f / rl[r];
                     }
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
-                        const int col = 64 * w + 16 * c + l16;
+                        const int col = 64 * w + 16 * c + (elane & 15);
                         if (col < kv) dst[col] = (acc[c][mt][i] + acc[c][mt][i + 2]) * f;
                     }
                 }
