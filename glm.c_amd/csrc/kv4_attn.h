@@ -1,12 +1,14 @@
 // kv4_attn.h -- MLA attention of a step's tokens over the paged cache in 4 bits (gmoe_kv4_attend).
 //
-// Work split. A request's fresh tokens times heads are its query rows; a tile is 8 MT of them
-// (MT 1, 2 or 3), and an item is a tile against a chunk of the request's positions. All chunks of a launch are
-// one length, a multiple of KA_P positions, the least that makes at most KA_ITEMS items beside
-// the one a tile needs (ka_plan): few long requests are cut fine, many are not cut at all. The
-// lengths are device data, so every block works out the split by itself from the requests'
-// lengths, and the grid is a fixed number of blocks that walk the items. A tile of one chunk is
-// written where it belongs; the others leave partial results that k_kv4_merge joins.
+// Work split. A request's fresh tokens times heads are its query rows; a tile is 8 MT of them (MT 1, 2
+// or 3) and a unit a tile against KA_P positions. All units of a launch lie on one axis, tile after
+// tile, each tile led by KA_LEAD for what it costs to begin one; the axis is cut into one equal
+// share a block, so that every block has the same work whatever the lengths. A tile inside one
+// share is written where it belongs; one that the cuts part leaves a partial result a block, which k_kv4_merge joins. A
+// block has at most two partial results, of its first tile and its last. The lengths are device data,
+// so every block works out the axis by itself; a tile's place on it is a formula (ka_place),
+// near its units' number, and the units in a share follow from the place alone (ka_cut), so that
+// neighbours agree.
 //
 // Products. Both run on v_mfma_f32_16x16x32_f16. The cache's values are exact in fp16 (e2m1 times a
 // power of two that the format holds to fp16's range), so only the queries and the exponentials
@@ -14,7 +16,7 @@
 // take three. The two parts of eight rows make the 16 operand rows of a tile, in the order
 // (hi hi lo lo) of rows 2g, 2g + 1: then a row's two sums lie in the same lane.
 //
-// A block (8 waves, one a CU) takes KA_P = 64 positions at a time:
+// A block (8 waves, one block a CU) takes KA_P = 64 positions at a time:
 //   scores   wave (h, g) has half h of the columns (nine blocks of 32) and positions 16 g .. + 15. A lane
 //            loads 16 bytes, a block of 32 codes, which are four steps' operands when the steps run over
 //            the blocks' eighths (the sum over columns may run in any order); v_cvt_scalef32_pk_f16_fp4
@@ -23,8 +25,9 @@
 //   softmax  wave w has rows 3 w .. + 2, a lane a position; the exponentials go to shared memory as
 //            operands.
 //   values   wave w has columns 64 w .. + 63: the rows of halves through the transposing read.
-// The values of a tile and the scores of the next share a phase, so two barriers a tile; codes
-// are requested a tile ahead, pages two.
+// The softmax of a tile and the scores of the next share a phase, in opposite order on the two waves of
+// a SIMD, so that the one's vector instructions run beside the other's matrix instructions; two barriers
+// a tile. Codes are requested a tile ahead, their pages two.
 //
 // Softmax reference: exponentials are taken against a row's reference, which follows the running
 // maximum only when a score passes it by 2^KA_SLACK, so that sums are rescaled a few times a
@@ -39,115 +42,128 @@
 #define KA_WAVES (KA_BLOCK / 64)
 #define KA_ROWS 24    // rows of the largest tile
 #define KA_HALF 9     // column blocks of a wave's half
-#define KA_GRID 256
-#define KA_ITEMS 512
-#define KA_MAX_PARTS (2 * KA_ITEMS)  // a cut tile has over U/c + 1 <= 2 U/c chunks, U/c of all at most KA_ITEMS
+#define KA_GRID 256   // blocks: one a CU
+#ifndef KA_SHARE
+#define KA_SHARE 2    // least share of a block
+#endif
+#define KA_LEAD 2
 #define KA_SLACK 6.0f
 #define KA_UP 8
-#define KA_VROW 528  // halves of a row of values in shared memory: rows 8 banks apart (of 64)
-#define KA_SROW 26   // floats of a position's scores
-#define KA_PROW 72   // halves of an operand row of exponentials
+#define KA_VROW 512  // halves of a row of values in shared memory
+#define KA_SROW 24   // floats of a position's scores
+#define KA_PROW 64   // halves of an operand row of exponentials
 #define KA_QROW 584  // halves of an operand row of queries (while they are staged)
 static_assert(2 * KA_HALF >= KV4_BLOCKS_MAX, "two halves hold a row");
 static_assert(2 * KA_ROWS * KA_QROW <= 2 * KA_P * KA_VROW, "the queries are staged where the values come later");
+
+// What a block leaves for k_kv4_merge: the cut tile that ends in its share (k > 1 partial results).
+struct KaCut {
+    int k;           // 0: none
+    int first, next; // slots of its partial results: first, next, next + 2, next + 4, ...
+    int t0, row0, nr;
+};
 
 struct Kv4Attn {
     Kv4Cache c;
     int R, max_pages, H;
     float scale;
+    double slope;    // units that a tile has more than the one before it, halved: rows / (2 KA_P H)
     const int32_t *table, *offsets, *context;
     const float *q_abs, *q_pe;
     int64_t ld_q_abs, ld_q_pe, ld_out;
     float *out;
-    float *part;     // [KA_MAX_PARTS][KA_ROWS][kv]
-    float *part_ml;  // [KA_MAX_PARTS][KA_ROWS][2]: a chunk's reference (of base 2, to a constant) and its sum of exponentials
+    float *part;     // [2 KA_GRID][KA_ROWS][kv]
+    float *part_ml;  // [2 KA_GRID][KA_ROWS][2]: a part's reference (of base 2, to a constant) and its sum of exponentials
+    KaCut *cuts;     // [KA_GRID]
 };
 
 // ---- the split of a launch -------------------------------------------------------------------
 
-__device__ static inline unsigned ka_tiles(const Kv4Attn &a, int r, int rows) {
-    const int fresh = a.offsets[r + 1] - a.offsets[r];
-    return fresh > 0 ? (unsigned)(fresh * a.H + rows - 1) / rows : 0u;  // (fresh * H < 2^27)
+__device__ static inline int ka_fresh(const Kv4Attn &a, int r) { return max(0, a.offsets[r + 1] - a.offsets[r]); }
+__device__ static inline unsigned ka_tiles(const Kv4Attn &a, int fresh, int rows) { return (unsigned)(fresh * a.H + rows - 1) / rows; }  // (fresh * H < 2^27)
+
+// The place on the axis of tile i of a request whose first token has `first` positions before it: a
+// trapezoid's area, rounded, so that it needs no sum over the tiles. Rises by over KA_LEAD a tile.
+__device__ static inline uint64_t ka_place(const Kv4Attn &a, uint64_t i, int first) {
+    return i * (KA_LEAD + 1) + i * (unsigned)max(0, first) / KA_P + (uint64_t)((double)(i * i) * a.slope);
 }
-__device__ static inline unsigned ka_units(const Kv4Attn &a, int r) {
-    const long long n = min((long long)a.context[r], (long long)a.max_pages << a.c.shift);  // what the table names
-    return n > 0 ? ((unsigned)n + KA_P - 1) / KA_P : 0u;
+// The units before place x of a tile of n units at place p, whose next tile is at e.
+__device__ static inline int ka_cut(uint64_t x, uint64_t p, uint64_t e, int n) {
+    return x >= e ? n : x <= p + KA_LEAD ? 0 : (int)min((uint64_t)n, x - p - KA_LEAD);
 }
 
-// A thread's share of the requests, and what lies before it. Cut tiles are those of more than one chunk.
+// A thread's requests and their place on the axis.
 struct KaPlan {
     int r0, r1;
-    unsigned items0, items, cuts0, cuts, parts0;
-    unsigned chunk, total, total_cuts;  // units of a chunk; all items; all cut tiles
+    uint64_t at, size;    // of its requests
+    uint64_t total, share;
 };
 struct KaShared {
-    unsigned red[KA_WAVES];
-    unsigned long long red2[KA_WAVES];
+    uint64_t red[KA_WAVES];
 };
 
-__device__ static inline unsigned ka_chunks(unsigned units, unsigned chunk) { return max(1u, (units + chunk - 1) / chunk); }
-
 __device__ static inline KaPlan ka_plan(const Kv4Attn &a, int rows, KaShared &sh) {
-    const int tid = threadIdx.x, nw = blockDim.x >> 6, per = (a.R + blockDim.x - 1) / blockDim.x;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, per = (a.R + KA_BLOCK - 1) / KA_BLOCK;
     KaPlan p;
     p.r0 = min(a.R, tid * per);
     p.r1 = min(a.R, p.r0 + per);
-    unsigned long long work = 0;
-    for (int r = p.r0; r < p.r1; r++) work += (unsigned long long)ka_tiles(a, r, rows) * ka_units(a, r);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) work += __shfl_xor(work, d);
-    if ((tid & 63) == 0) sh.red2[tid >> 6] = work;
-    __syncthreads();
-    work = 0;
-    for (int i = 0; i < nw; i++) work += sh.red2[i];
-    p.chunk = (unsigned)max(1ull, min((work + KA_ITEMS - 1) / KA_ITEMS, 1ull << 30));
-    p.items = p.cuts = 0;
-    unsigned parts = 0;
+    p.size = 0;
     for (int r = p.r0; r < p.r1; r++) {
-        const unsigned t = ka_tiles(a, r, rows), k = ka_chunks(ka_units(a, r), p.chunk);
-        p.items += t * k;
-        if (k > 1) {
-            p.cuts += t;
-            parts += t * k;
-        }
+        const int fresh = ka_fresh(a, r);
+        p.size += ka_place(a, ka_tiles(a, fresh, rows), a.context[r] - fresh);
     }
-    unsigned n;
-    p.items0 = block_scan_u(p.items, sh.red, &p.total);
-    p.cuts0 = block_scan_u(p.cuts, sh.red, &p.total_cuts);
-    p.parts0 = block_scan_u(parts, sh.red, &n);
+    uint64_t s = p.size;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint64_t o = __shfl_up(s, d);
+        if (lane >= d) s += o;
+    }
+    if (lane == 63) sh.red[w] = s;
+    __syncthreads();
+    p.at = s - p.size;
+    p.total = 0;
+#pragma unroll
+    for (int i = 0; i < KA_WAVES; i++) {
+        if (i < w) p.at += sh.red[i];
+        p.total += sh.red[i];
+    }
+    p.share = max((uint64_t)KA_SHARE, (p.total + KA_GRID - 1) / KA_GRID);
     return p;
 }
 
-// One item of the split.
+// A tile, and its place.
 struct KaItem {
-    int r, tile, k, chunk;     // request, tile of it, its chunks, this one
-    int t0, fresh, context;    // the request's first token, its tokens, its positions
-    unsigned part;             // partial-result slot of the item (k > 1)
+    int r, tile, t0, fresh, context;  // request, tile of it; the request's first token, its tokens, its positions
+    uint64_t p, e;
 };
 
-// The item of number `i` (of the cut tiles, first chunk, when CUT) by the thread that has it.
-template <bool CUT>
-__device__ static inline void ka_find(const Kv4Attn &a, const KaPlan &p, int rows, unsigned i, KaItem *out) {
-    const unsigned base = CUT ? p.cuts0 : p.items0, mine = CUT ? p.cuts : p.items;
-    if (i - base >= mine) return;
-    unsigned left = i - base, part = p.parts0;
+// The tile at place x, by the thread that has its request.
+__device__ static inline void ka_find(const Kv4Attn &a, const KaPlan &p, int rows, uint64_t x, KaItem *out) {
+    if (x - p.at >= p.size) return;
+    uint64_t at = p.at;
     for (int r = p.r0; r < p.r1; r++) {
-        const unsigned t = ka_tiles(a, r, rows), k = ka_chunks(ka_units(a, r), p.chunk), n = CUT ? (k > 1 ? t : 0) : t * k;
-        if (left < n) {
+        const int fresh = ka_fresh(a, r), first = a.context[r] - fresh;
+        const uint64_t n = ka_tiles(a, fresh, rows), size = ka_place(a, n, first);
+        if (x - at < size) {
+            // the last tile whose place is at most x - at, by halving
+            uint64_t lo = 0, hi = n;
+            while (hi - lo > 1) {
+                const uint64_t mid = (lo + hi) >> 1;
+                if (ka_place(a, mid, first) <= x - at) lo = mid;
+                else hi = mid;
+            }
             KaItem m;
             m.r = r;
-            m.k = (int)k;
-            m.tile = (int)(CUT ? left : left / k);
-            m.chunk = (int)(CUT ? 0 : left % k);
+            m.tile = (int)lo;
             m.t0 = a.offsets[r];
-            m.fresh = a.offsets[r + 1] - m.t0;
+            m.fresh = fresh;
             m.context = max(0, a.context[r]);
-            m.part = part + m.tile * k + m.chunk;
+            m.p = at + ka_place(a, lo, first);
+            m.e = at + ka_place(a, lo + 1, first);
             *out = m;
             return;
         }
-        left -= n;
-        if (k > 1) part += t * k;
+        at += size;
     }
 }
 
@@ -184,9 +200,12 @@ template <int MT>
 __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
     constexpr int ROWS = 8 * MT, OPS = 16 * MT, RPW = MT;  // rows, operand rows, rows of a wave's softmax
     static_assert(RPW * KA_WAVES == ROWS, "every row has a wave");
+    // Rows of 16-byte pieces, 16 pieces 256 bytes; piece i of a row lies at i ^ (a number of the row), so that
+    // neither the eight rows that are written side by side nor the eight that the transposing read takes
+    // a pair of pieces from meet in a bank
     __shared__ __align__(16) _Float16 val[2][KA_P * KA_VROW];
-    __shared__ __align__(16) float sc[2][KA_P][KA_SROW];
-    __shared__ __align__(16) _Float16 pr[OPS][KA_PROW];
+    __shared__ __align__(16) float sc[2][2][KA_P * KA_SROW];
+    __shared__ __align__(16) _Float16 pr[OPS * KA_PROW];
     __shared__ __align__(8) float cr[ROWS], rl[ROWS], rm[ROWS];
     __shared__ __align__(8) unsigned char moved[KA_WAVES];
     __shared__ KaShared sh;
@@ -195,20 +214,27 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
     const int kv = a.c.kv, rope = a.c.rope, nb = a.c.blocks, shift = a.c.shift;
     const KaPlan plan = ka_plan(a, ROWS, sh);
     const float scale = __fmul_rn(a.scale, 1.44269504f);  // scores of base 2
+    const uint64_t x0 = blockIdx.x * plan.share, x1 = min(plan.total, x0 + plan.share);
+    if (threadIdx.x == 0) a.cuts[blockIdx.x].k = 0;
 
-    for (unsigned it = blockIdx.x; it < plan.total; it += gridDim.x) {
+    for (uint64_t at = x0; at < x1;) {
         __syncthreads();
-        ka_find<false>(a, plan, ROWS, it, &item);
+        ka_find(a, plan, ROWS, at, &item);
         __syncthreads();
         const KaItem m = item;
+        at = m.e;
         const int rows = m.fresh * a.H, row0 = m.tile * ROWS, nr = min(ROWS, rows - row0);
         const int first = m.context - m.fresh;  // the position of the request's first token
         const int end = (int)min((long long)max(0, first + min(m.fresh, (row0 + nr - 1) / a.H + 1)), (long long)a.max_pages << shift);
-        const long long c0 = (long long)m.chunk * plan.chunk * KA_P;
-        const int s0 = (int)min(c0, (long long)end), s1 = (int)min(c0 + (long long)plan.chunk * KA_P, (long long)end);
-        const int nt = (s1 - s0 + KA_P - 1) / KA_P;
+        const int units = (end + KA_P - 1) / KA_P;
+        const int u0 = ka_cut(x0, m.p, m.e, units), u1 = ka_cut(x1, m.p, m.e, units);
+        // the places of its first unit and its last; the block that has the one and the other has it whole
+        const uint64_t head = units > 0 ? m.p + KA_LEAD : m.p, tail = units > 0 ? min(m.p + KA_LEAD + units, m.e) - 1 : m.p;
+        const bool ends = x0 <= tail && tail < x1, whole = ends && x0 <= head;
+        if (units > 0 ? u0 == u1 : !whole) continue;
+        const int s0 = KA_P * u0, s1 = min(end, KA_P * u1), nt = u1 - u0;
+        const int slot = 2 * blockIdx.x + (m.p > x0 ? 1 : 0);  // of a partial result: the block's first tile, or its last
         const int32_t *table = a.table + (size_t)m.r * a.max_pages;
-
         const int tid = ka_tid(), lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
         // The lane's blocks of its half, and which of the half's bytes are their scales. A block past the
         // row's last reads codes of another at scale 0.
@@ -219,6 +245,7 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
         // (a row ends 16 bytes past its codes, 32 where it has over 16 blocks)
         const int ats = 16 * nb + (KA_HALF * kh < nb ? 8 * kh : 0), atw = 16 * nb + (kh == 0 ? 8 : nb > 16 ? 16 : 0);
         const bool v0 = 32 * b0 < kv, v1 = 32 * b1 < kv, v2 = 32 * b2 < kv;  // blocks of the entry, not of the rope part
+
         // the lane's position of tile j: its page, as the table has it (nothing looks at it before fetch(),
         // so that nothing waits for it), and from the page its row
         auto page_of = [&](int j) { return *gbl(table + (min(s0 + KA_P * j + 16 * pg + l16, s1 - 1) >> shift)); };
@@ -292,6 +319,13 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
             for (int mt = 0; mt < MT; mt++) acc[c][mt] = (aq_f4){0.0f, 0.0f, 0.0f, 0.0f};
         __syncthreads();  // the staged queries are read; values may come
 
+        // where the lane writes values (pieces 4 b0 .. + 3, then b1's 16 on, and its eighth of block 2) and scores
+        const int mix = (2 * (l16 & 7)) ^ (l16 >> 2 & 1);
+        int wat[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) wat[k] = 8 * ((4 * b0 + k) ^ mix);
+        const int wat2 = 8 * ((4 * b2 + lg) ^ mix);
+        const int sat = (16 * pg + l16) * KA_SROW + ((2 * lg) ^ (l16 & 8) >> 1 ^ (pg & 1) << 1);
         // tile j's scores (this half's part) from `raw`, its values to shared memory
         auto scores = [&](int j) {
             unsigned e0 = __builtin_amdgcn_perm(raw.w0[1], raw.w0[0], sel0) & raw.on, e1 = __builtin_amdgcn_perm(raw.w1, raw.w0[1], sel1) & raw.on,
@@ -305,10 +339,7 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
                 spoilt |= spoilt >> 16;
             }
             const float f0 = __uint_as_float(e0 << 23), f1 = __uint_as_float(e1 << 23), f2 = __uint_as_float(e2 << 23);
-            const int p = 16 * pg + l16;
-            // rows r and r + 8 have the halves of 16 columns the other way round, in other banks
-            _Float16 *dst = val[j & 1] + p * KA_VROW;
-            const int flip = p & 8;
+            _Float16 *dst = val[j & 1] + (16 * pg + l16) * KA_VROW;
             aq_f4 d[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) d[mt] = (aq_f4){0.0f, 0.0f, 0.0f, 0.0f};
@@ -317,18 +348,16 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
                 a16_h8 x[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) x[k] = ka_halves(g ? raw.q1[k] : raw.q0[k], g ? f1 : f0);
-                if (g ? v1 : v0) {
-                    _Float16 *at = dst + 32 * (g ? b1 : b0);
+                if (g ? v1 : v0)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) *(a16_h8 *)(at + ((8 * k) ^ flip)) = x[k];
-                }
+                    for (int k = 0; k < 4; k++) *(a16_h8 *)(dst + wat[k] + 128 * g) = x[k];
 #pragma unroll
                 for (int k = 0; k < 4; k++)
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) d[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[4 * g + k][mt], x[k], d[mt], 0, 0, 0);
             }
             const a16_h8 x = ka_halves(raw.q2, f2);
-            if (v2) *(a16_h8 *)(dst + 32 * b2 + ((8 * lg) ^ flip)) = x;
+            if (v2) *(a16_h8 *)(dst + wat2) = x;
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) d[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[8][mt], x, d[mt], 0, 0, 0);
             float2 t[MT];
@@ -341,18 +370,28 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
                     for (int mt = 0; mt < MT; mt++) t[mt] = make_float2(odd, odd);
             }
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) *(float2 *)&sc[kh][p][8 * mt + 2 * lg] = t[mt];
+            for (int mt = 0; mt < MT; mt++) *(float2 *)&sc[j & 1][kh][sat + 8 * mt] = t[mt];
         };
         // tile j's exponentials from its scores
-        const int slot_at = 32 * (lane >> 5) + 8 * ((lane & 15) >> 2) + 4 * ((lane & 31) >> 4) + (lane & 3);  // a position's operand slot
-        _Float16 *const pdst = &pr[0][slot_at];
+        int rat[RPW];          // the lane's position's score of its rows
+        _Float16 *pat[RPW];    // the operand that the lane writes: its pair of positions' first parts, or the second
+        {
+            const int op = 32 * (lane >> 5) + 8 * ((lane & 15) >> 2) + 4 * ((lane & 31) >> 4) + (lane & 2);  // the pair's operand slot
+#pragma unroll
+            for (int i = 0; i < RPW; i++) {
+                const int r = RPW * w + i, o = 16 * (r >> 3) + 4 * ((r & 7) >> 1) + (r & 1) + 2 * (lane & 1);
+                rat[i] = lane * KA_SROW + (r ^ (lane & 8) >> 1 ^ (lane & 16) >> 3);
+                pat[i] = pr + o * KA_PROW + (op ^ 8 * ((o & 7) ^ (o >> 3 & 1)));
+            }
+        }
+        const unsigned pick = lane & 1 ? 0x03020706u : 0x05040100u;  // of (the partner's, the lane's) pair of parts
         auto softmax = [&](int j) {
             const int s = s0 + KA_P * j + lane;
             float t[RPW];
             bool up[RPW], any = false;
 #pragma unroll
             for (int i = 0; i < RPW; i++) {
-                const float x = sc[0][lane][RPW * w + i] + sc[1][lane][RPW * w + i];
+                const float x = sc[j & 1][0][rat[i]] + sc[j & 1][1][rat[i]];
                 t[i] = ldexpf(x, eq[i]);
                 on[i] = s <= last[i] && x != -INFINITY;
                 up[i] = on[i] && t[i] * scale > top[i];
@@ -377,16 +416,24 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
             if (lane == 0) moved[w] = move;
 #pragma unroll
             for (int i = 0; i < RPW; i++) {
-                const int r = RPW * w + i;
                 const float ref = top[i] - (KA_SLACK + KA_UP);
                 const float e = on[i] ? __builtin_amdgcn_exp2f(fmaf(t[i], scale, -ref)) : 0.0f;
                 lsum[i] += e;
-                _Float16 *dst = pdst + (16 * (r >> 3) + 4 * ((r & 7) >> 1) + (r & 1)) * KA_PROW;
-                const _Float16 hi = (_Float16)e;
-                dst[0] = hi;
-                dst[2 * KA_PROW] = (_Float16)fmaf((float)hi, -1.0f, e);
+                ka_h2 both;
+                both.x = (_Float16)e;
+                both.y = (_Float16)fmaf((float)both.x, -1.0f, e);
+                const unsigned me = __builtin_bit_cast(unsigned, both), other = (unsigned)__builtin_amdgcn_update_dpp(0, (int)me, DPP_QUAD_1032, 0xF, 0xF, false);
+                *(unsigned *)pat[i] = __builtin_amdgcn_perm(other, me, pick);
             }
         };
+        // where the lane reads exponentials, and four rows' values of each 16 columns
+        const int pin = l16 * KA_PROW + 8 * (lg ^ (l16 & 7) ^ (l16 >> 3));
+        int vin[4];
+        {
+            const int row = 4 * lg + (l16 >> 2), m2 = (2 * (row & 7)) ^ (row >> 2 & 1);
+#pragma unroll
+            for (int c = 0; c < 4; c++) vin[c] = row * KA_VROW + 8 * ((8 * w + 2 * c + (l16 >> 1 & 1)) ^ m2) + 4 * (l16 & 1);
+        }
         // tile j's values weighted
         auto values = [&](int j) {
             const u32x2 mv = *(const u32x2 *)moved;
@@ -398,15 +445,15 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
                     for (int c = 0; c < 4; c++) acc[c][mt] *= (aq_f4){f.x, f.y, f.x, f.y};
                 }
             }
-            const _Float16 *src = val[j & 1] + (4 * lg + (l16 >> 2)) * KA_VROW + ((64 * w + 4 * (l16 & 3)) ^ (lg & 2 ? 8 : 0));
+            const _Float16 *src = val[j & 1];
 #pragma unroll
             for (int ks = 0; ks < KA_P / 32; ks++) {
                 a16_h8 p[MT];
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++) p[mt] = *(const a16_h8 *)&pr[16 * mt + l16][32 * ks + 8 * lg];
+                for (int mt = 0; mt < MT; mt++) p[mt] = *(const a16_h8 *)(pr + 16 * mt * KA_PROW + (ks ? pin ^ 32 : pin));
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    const a16_h4 x = a16_tr(src + 32 * ks * KA_VROW + 16 * c), y = a16_tr(src + (32 * ks + 16) * KA_VROW + 16 * c);
+                    const a16_h4 x = a16_tr(src + vin[c] + 32 * ks * KA_VROW), y = a16_tr(src + vin[c] + (32 * ks + 16) * KA_VROW);
                     const a16_h8 v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) acc[c][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[mt], v, acc[c][mt], 0, 0, 0);
@@ -414,21 +461,23 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
             }
         };
         const bool mine = 64 * w < kv;  // the wave has columns
+        auto ahead = [&](int j) {  // tile j's scores, and the request of the next one's codes
+            scores(j);
+            if (j + 1 < nt) {
+                fetch(raw, j + 1, page);
+                if (j + 2 < nt) page = page_of(j + 2);
+            }
+        };
         if (nt > 0) {
-            for (int j = 0; j <= nt; j++) {
-                if (j < nt) {
-                    scores(j);
-                    if (j + 1 < nt) {
-                        fetch(raw, j + 1, page);
-                        if (j + 2 < nt) page = page_of(j + 2);
-                    }
-                }
-                if (j > 0 && mine) values(j - 1);
+            ahead(0);
+            block_barrier();
+            for (int j = 0; j < nt; j++) {
+                if (kh == 0 && j + 1 < nt) ahead(j + 1);
+                softmax(j);
+                if (kh != 0 && j + 1 < nt) ahead(j + 1);
                 block_barrier();
-                if (j < nt) {
-                    softmax(j);
-                    block_barrier();
-                }
+                if (mine) values(j);
+                block_barrier();
             }
         }
         // the rows' sums to every wave, and the results
@@ -443,8 +492,12 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
             }
         }
         __syncthreads();
-        if (m.k > 1 && etid < nr) {
-            float *ml = a.part_ml + ((size_t)m.part * KA_ROWS + etid) * 2;
+        if (ends && !whole && etid == 0) {
+            const int bf = (int)(head / plan.share);  // the block of the first part
+            a.cuts[blockIdx.x] = KaCut{(int)blockIdx.x - bf + 1, 2 * bf + (m.p > bf * plan.share ? 1 : 0), 2 * bf + 2, m.t0, row0, nr};
+        }
+        if (!whole && etid < nr) {
+            float *ml = a.part_ml + ((size_t)slot * KA_ROWS + etid) * 2;
             ml[0] = rm[etid];
             ml[1] = rl[etid];
         }
@@ -457,8 +510,8 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
                     if (r >= nr) continue;
                     float *dst;
                     float f = 1.0f;
-                    if (m.k > 1) {
-                        dst = a.part + ((size_t)m.part * KA_ROWS + r) * kv;
+                    if (!whole) {
+                        dst = a.part + ((size_t)slot * KA_ROWS + r) * kv;
                     } else {
                         const int g = row0 + r, t = g / a.H;
                         dst = a.out + (m.t0 + t) * a.ld_out + (int64_t)(g - t * a.H) * kv;
@@ -474,82 +527,67 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
     }
 }
 
-// The cut tiles' partial results joined, a block a query row: out = sum_c w_c part_c / sum_c w_c l_c
-// with w_c = 2^(ref_c - max ref). Threads have four columns each; the groups that cover a row share
-// its chunks.
-__global__ __launch_bounds__(KA_BLOCK) void k_kv4_merge(Kv4Attn a, int rows) {
-    __shared__ KaShared sh;
-    __shared__ KaItem item;
-    __shared__ float wgt[KA_ITEMS];
-    __shared__ float red[KA_WAVES];
-    __shared__ __align__(16) float4 sum[KA_BLOCK];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, kv = a.c.kv;
-    const KaPlan plan = ka_plan(a, rows, sh);
-    const int cols = kv / 4, groups = KA_BLOCK / cols, grp = tid / cols, col = tid - grp * cols;
-    for (unsigned unit = blockIdx.x; unit < plan.total_cuts * rows; unit += gridDim.x) {
-        const unsigned ti = unit / rows;
-        const int rr = (int)(unit - ti * rows);
-        __syncthreads();
-        ka_find<true>(a, plan, rows, ti, &item);
-        __syncthreads();
-        const KaItem m = item;
-        const int g = m.tile * rows + rr;
-        if (g >= m.fresh * a.H) continue;
-        const float *ml = a.part_ml + ((size_t)m.part * KA_ROWS + rr) * 2;
-        float pm = -INFINITY, pl = 0.0f;
-        if (tid < m.k) {
-            pm = ml[(size_t)tid * KA_ROWS * 2];
-            pl = ml[(size_t)tid * KA_ROWS * 2 + 1];
-        }
-        const float wm = wave_max_dpp_f(pm);
-        if (lane == 0) red[w] = wm;
-        __syncthreads();
-        float mx = red[0];
-#pragma unroll
-        for (int i = 1; i < KA_WAVES; i++) mx = fmaxf(mx, red[i]);
-        __syncthreads();
-        const float e = pl == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(pm - mx);
-        if (tid < m.k) wgt[tid] = e;
-        float l = row_sum_dpp_f(e * pl);
-        l = (readlane_f(l, 0) + readlane_f(l, 16)) + (readlane_f(l, 32) + readlane_f(l, 48));
-        if (lane == 0) red[w] = l;
-        __syncthreads();
-        l = 0.0f;
-#pragma unroll
-        for (int i = 0; i < KA_WAVES; i++) l += red[i];
-        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (grp < groups) {
-            const float *pc = a.part + ((size_t)m.part * KA_ROWS + rr) * kv + 4 * col;
-#pragma unroll 4
-            for (int c = grp; c < m.k; c += groups) {
-                const float4 v = *(const float4 *)(pc + (size_t)c * KA_ROWS * kv);
-                const float x = wgt[c];
-                s.x = fmaf(x, v.x, s.x);
-                s.y = fmaf(x, v.y, s.y);
-                s.z = fmaf(x, v.z, s.z);
-                s.w = fmaf(x, v.w, s.w);
-            }
-        }
-        sum[tid] = s;
-        __syncthreads();
-        if (tid < cols) {
-            for (int k = 1; k < groups; k++) {
-                const float4 v = sum[tid + k * cols];
-                s.x += v.x;
-                s.y += v.y;
-                s.z += v.z;
-                s.w += v.w;
-            }
-            const int t = g / a.H;
-            float *dst = a.out + (m.t0 + t) * a.ld_out + (int64_t)(g - t * a.H) * kv + 4 * tid;
-            const float f = l == 0.0f ? 0.0f : 1.0f / l;
-            dst[0] = s.x * f;
-            dst[1] = s.y * f;
-            dst[2] = s.z * f;
-            dst[3] = s.w * f;
+// The cut tiles' partial results joined: out = sum_c w_c part_c / sum_c w_c l_c with w_c = 2^(ref_c - max
+// ref). A block has two rows of the tile that ends in share blockIdx.y; a row's threads have four columns
+// each and every other part.
+#define KM_ROWS 2
+#define KM_GROUPS 2
+#define KM_COLS (KA_BLOCK / KM_ROWS / KM_GROUPS)
+static_assert(4 * KM_COLS >= 512, "a group's threads cover a row");
+__global__ __launch_bounds__(KA_BLOCK) void k_kv4_merge(Kv4Attn a) {
+    __shared__ float wgt[KM_ROWS][KA_GRID];
+    __shared__ float red[KM_ROWS][KA_WAVES / KM_ROWS], red2[KM_ROWS][KA_WAVES / KM_ROWS];
+    __shared__ __align__(16) float4 sum[KM_ROWS][KM_COLS];
+    const KaCut m = a.cuts[blockIdx.y];
+    const int kv = a.c.kv, tid = threadIdx.x;
+    const int sub = __builtin_amdgcn_readfirstlane(tid / (KA_BLOCK / KM_ROWS)), t = tid % (KA_BLOCK / KM_ROWS), rr = blockIdx.x * KM_ROWS + sub;
+    if (m.k == 0 || (int)blockIdx.x * KM_ROWS >= m.nr) return;
+    const bool there = rr < m.nr;
+    auto at = [&](int c) { return (size_t)(c == 0 ? m.first : m.next + 2 * (c - 1)) * KA_ROWS + rr; };
+    static_assert(KA_GRID <= KA_BLOCK / KM_ROWS, "a thread a part");
+    float pm = -INFINITY, pl = 0.0f;
+    if (there && t < m.k) {
+        pm = a.part_ml[at(t) * 2];
+        pl = a.part_ml[at(t) * 2 + 1];
+    }
+    const float wm = wave_max_dpp_f(pm);
+    if ((t & 63) == 0) red[sub][t >> 6] = wm;
+    __syncthreads();
+    const float mx = fmaxf(fmaxf(red[sub][0], red[sub][1]), fmaxf(red[sub][2], red[sub][3]));
+    const float e = pl == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(pm - mx);
+    if (t < m.k) wgt[sub][t] = e;
+    float l = row_sum_dpp_f(pl == 0.0f ? 0.0f : e * pl);
+    l = (readlane_f(l, 0) + readlane_f(l, 16)) + (readlane_f(l, 32) + readlane_f(l, 48));
+    if ((t & 63) == 0) red2[sub][t >> 6] = l;
+    __syncthreads();
+    l = (red2[sub][0] + red2[sub][1]) + (red2[sub][2] + red2[sub][3]);
+    const int grp = t / KM_COLS, col = 4 * (t % KM_COLS);
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (there && col < kv) {
+#pragma unroll 8
+        for (int c = grp; c < m.k; c += KM_GROUPS) {
+            const float4 v = *(const float4 *)(a.part + at(c) * kv + col);
+            const float x = wgt[sub][c];
+            s.x = fmaf(x, v.x, s.x);
+            s.y = fmaf(x, v.y, s.y);
+            s.z = fmaf(x, v.z, s.z);
+            s.w = fmaf(x, v.w, s.w);
         }
     }
+    if (grp == 1) sum[sub][t % KM_COLS] = s;
+    __syncthreads();
+    if (there && col < kv && grp == 0) {
+        const float4 v = sum[sub][t];
+        const int g = m.row0 + rr, tok = g / a.H;
+        float *dst = a.out + (m.t0 + tok) * a.ld_out + (int64_t)(g - tok * a.H) * kv + col;
+        const float f = l == 0.0f ? 0.0f : 1.0f / l;
+        dst[0] = (s.x + v.x) * f;
+        dst[1] = (s.y + v.y) * f;
+        dst[2] = (s.z + v.z) * f;
+        dst[3] = (s.w + v.w) * f;
+    }
 }
+static_assert(KM_GROUPS == 2 && KA_WAVES / KM_ROWS == 4, "two groups, four waves a row");
 
 // Operand tiles a row tile for rows of a request's step, by the cost of the tiles it takes: each
 // converts the cache's codes once (about one operand tile's products) and multiplies MT operand tiles.

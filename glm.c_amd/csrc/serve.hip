@@ -145,7 +145,7 @@ extern "C" int gmoe_kv4_read(int device, const gmoe_kv4 *c, int n, const int32_t
 
 extern "C" size_t gmoe_kv4_attend_workspace(int n_heads, int kv_lora_rank) {
     if (n_heads < 1 || n_heads > 256 || !ranks_ok(kv_lora_rank, 2)) return 0;
-    return (size_t)KA_MAX_PARTS * KA_ROWS * (kv_lora_rank + 2) * sizeof(float);
+    return (size_t)2 * KA_GRID * KA_ROWS * (kv_lora_rank + 2) * sizeof(float) + KA_GRID * sizeof(KaCut);
 }
 
 extern "C" int gmoe_kv4_attend(int device, const gmoe_kv4 *c, const gmoe_batch *b, const gmoe_kv4_heads *h, void *stream) {
@@ -179,16 +179,18 @@ extern "C" int gmoe_kv4_attend(int device, const gmoe_kv4 *c, const gmoe_batch *
     a.out = h->out;
     a.ld_out = h->ld_out;
     a.part = (float *)h->work;
-    a.part_ml = a.part + (size_t)KA_MAX_PARTS * KA_ROWS * a.c.kv;
+    a.part_ml = a.part + (size_t)2 * KA_GRID * KA_ROWS * a.c.kv;
+    a.cuts = (KaCut *)(a.part_ml + (size_t)2 * KA_GRID * KA_ROWS * 2);
     OnDevice on(device);
     if (on.err != hipSuccess) return failed("gmoe_kv4_attend: the device", on.err);
     hipStream_t st = (hipStream_t)stream;
     // the host knows no request's tokens: it takes them all alike
     const int mt = ka_operand_tiles((long long)a.H * ((b->max_tokens + a.R - 1) / a.R));
+    a.slope = 8.0 * mt / (2.0 * KA_P * a.H);
     if (mt == 1) hipLaunchKernelGGL(k_kv4_attend<1>, dim3(KA_GRID), dim3(KA_BLOCK), 0, st, a);
     else if (mt == 2) hipLaunchKernelGGL(k_kv4_attend<2>, dim3(KA_GRID), dim3(KA_BLOCK), 0, st, a);
     else hipLaunchKernelGGL(k_kv4_attend<3>, dim3(KA_GRID), dim3(KA_BLOCK), 0, st, a);
-    hipLaunchKernelGGL(k_kv4_merge, dim3(KA_GRID), dim3(KA_BLOCK), 0, st, a, 8 * mt);
+    hipLaunchKernelGGL(k_kv4_merge, dim3(8 * mt / KM_ROWS, KA_GRID), dim3(KA_BLOCK), 0, st, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? GMOE_OK : failed("gmoe_kv4_attend", e);
 }
