@@ -43,10 +43,8 @@
 #define KA_ROWS 24    // rows of the largest tile
 #define KA_HALF 9     // column blocks of a wave's half
 #define KA_GRID 256   // blocks: one a CU
-#ifndef KA_SHARE
-#define KA_SHARE 2    // least share of a block
-#endif
-#define KA_LEAD 2
+#define KA_SHARE 2    // least share of a block: with 1 a token at 4096 takes 14.2 + 6.4 us (the join), with 2 15.6 + 5.0
+#define KA_LEAD 4     // of a tile's beginning, in units (64 ragged requests: 39 us with 2, 32 with 4, 34 with 7)
 #define KA_SLACK 6.0f
 #define KA_UP 8
 #define KA_VROW 512  // halves of a row of values in shared memory
@@ -79,7 +77,6 @@ struct Kv4Attn {
 
 // ---- the split of a launch -------------------------------------------------------------------
 
-__device__ static inline int ka_fresh(const Kv4Attn &a, int r) { return max(0, a.offsets[r + 1] - a.offsets[r]); }
 __device__ static inline unsigned ka_tiles(const Kv4Attn &a, int fresh, int rows) { return (unsigned)(fresh * a.H + rows - 1) / rows; }  // (fresh * H < 2^27)
 
 // The place on the axis of tile i of a request whose first token has `first` positions before it: a
@@ -92,85 +89,116 @@ __device__ static inline int ka_cut(uint64_t x, uint64_t p, uint64_t e, int n) {
     return x >= e ? n : x <= p + KA_LEAD ? 0 : (int)min((uint64_t)n, x - p - KA_LEAD);
 }
 
-// A thread's requests and their place on the axis.
-struct KaPlan {
-    int r0, r1;
-    uint64_t at, size;    // of its requests
-    uint64_t total, share;
-};
-struct KaShared {
-    uint64_t red[KA_WAVES];
-};
-
-__device__ static inline KaPlan ka_plan(const Kv4Attn &a, int rows, KaShared &sh) {
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, per = (a.R + KA_BLOCK - 1) / KA_BLOCK;
-    KaPlan p;
-    p.r0 = min(a.R, tid * per);
-    p.r1 = min(a.R, p.r0 + per);
-    p.size = 0;
-    for (int r = p.r0; r < p.r1; r++) {
-        const int fresh = ka_fresh(a, r);
-        p.size += ka_place(a, ka_tiles(a, fresh, rows), a.context[r] - fresh);
-    }
-    uint64_t s = p.size;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = __shfl_up(s, d);
-        if (lane >= d) s += o;
-    }
-    if (lane == 63) sh.red[w] = s;
-    __syncthreads();
-    p.at = s - p.size;
-    p.total = 0;
-#pragma unroll
-    for (int i = 0; i < KA_WAVES; i++) {
-        if (i < w) p.at += sh.red[i];
-        p.total += sh.red[i];
-    }
-    p.share = max((uint64_t)KA_SHARE, (p.total + KA_GRID - 1) / KA_GRID);
-    return p;
-}
-
 // A tile, and its place.
 struct KaItem {
     int r, tile, t0, fresh, context;  // request, tile of it; the request's first token, its tokens, its positions
     uint64_t p, e;
 };
 
-// The tile at place x, by the thread that has its request.
-__device__ static inline void ka_find(const Kv4Attn &a, const KaPlan &p, int rows, uint64_t x, KaItem *out) {
-    if (x - p.at >= p.size) return;
-    uint64_t at = p.at;
+// The axis of a launch. With at most 64 requests every wave has them all, a lane each, and finds
+// tiles by itself; with more a thread of the block has every KA_BLOCK-th run of them, and the one that
+// has a tile hands it over in shared memory.
+struct KaPlan {
+    int r0, r1;                   // the thread's requests
+    int t0, fresh, context;       // of the first
+    double at, size;              // their place on the axis (whole numbers below 2^53)
+    uint64_t total, share;
+};
+struct KaShared {
+    double red[KA_WAVES];
+    KaItem item;
+};
+
+__device__ static inline double ka_size(const Kv4Attn &a, int fresh, int context, int rows) {
+    return (double)ka_place(a, ka_tiles(a, fresh, rows), context - fresh);
+}
+
+__device__ static inline KaPlan ka_plan(const Kv4Attn &a, int rows, KaShared &sh) {
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const bool few = a.R <= 64;
+    const int per = few ? 1 : (a.R + KA_BLOCK - 1) / KA_BLOCK, mine = few ? lane : tid;
+    KaPlan p;
+    p.r0 = min(a.R, mine * per);
+    p.r1 = min(a.R, p.r0 + per);
+    p.t0 = p.fresh = p.context = 0;
+    p.size = 0.0;
     for (int r = p.r0; r < p.r1; r++) {
-        const int fresh = ka_fresh(a, r), first = a.context[r] - fresh;
-        const uint64_t n = ka_tiles(a, fresh, rows), size = ka_place(a, n, first);
-        if (x - at < size) {
-            // the last tile whose place is at most x - at, by halving
-            uint64_t lo = 0, hi = n;
-            while (hi - lo > 1) {
-                const uint64_t mid = (lo + hi) >> 1;
-                if (ka_place(a, mid, first) <= x - at) lo = mid;
-                else hi = mid;
-            }
-            KaItem m;
-            m.r = r;
-            m.tile = (int)lo;
-            m.t0 = a.offsets[r];
-            m.fresh = fresh;
-            m.context = max(0, a.context[r]);
-            m.p = at + ka_place(a, lo, first);
-            m.e = at + ka_place(a, lo + 1, first);
-            *out = m;
-            return;
+        const int t0 = a.offsets[r], fresh = max(0, a.offsets[r + 1] - t0), context = a.context[r];
+        if (r == p.r0) {
+            p.t0 = t0;
+            p.fresh = fresh;
+            p.context = context;
         }
-        at += size;
+        p.size += ka_size(a, fresh, context, rows);
     }
+    const double s = wave_incl_scan_dpp(p.size);
+    double before = 0.0, total = readlane_d(s, 63);
+    if (!few) {
+        if (lane == 63) sh.red[w] = s;
+        __syncthreads();
+        total = 0.0;
+#pragma unroll
+        for (int i = 0; i < KA_WAVES; i++) {
+            if (i < w) before += sh.red[i];
+            total += sh.red[i];
+        }
+    }
+    p.at = before + s - p.size;
+    p.total = (uint64_t)readlane_d(total, 0);
+    p.share = max((uint64_t)KA_SHARE, (p.total + KA_GRID - 1) / KA_GRID);
+    return p;
+}
+
+// The tile of a request, from place `at` on, that has place x.
+__device__ static inline KaItem ka_tile(const Kv4Attn &a, int rows, uint64_t x, int r, int t0, int fresh, int context, uint64_t at) {
+    uint64_t lo = 0, hi = ka_tiles(a, fresh, rows);
+    while (hi - lo > 1) {  // the last tile whose place is at most x, by halving
+        const uint64_t mid = (lo + hi) >> 1;
+        if (at + ka_place(a, mid, context - fresh) <= x) lo = mid;
+        else hi = mid;
+    }
+    return KaItem{r, (int)lo, t0, fresh, max(0, context), at + ka_place(a, lo, context - fresh), at + ka_place(a, lo + 1, context - fresh)};
+}
+
+// The tile at place x, to every thread of the block.
+__device__ static inline KaItem ka_find(const Kv4Attn &a, const KaPlan &p, int rows, uint64_t x, KaShared &sh) {
+    const double d = (double)x;
+    const bool has = d >= p.at && d < p.at + p.size;
+    if (a.R <= 64) {
+        const int l = __ffsll(__ballot(has)) - 1;
+        return ka_tile(a, rows, x, l, __builtin_amdgcn_readlane(p.t0, l), __builtin_amdgcn_readlane(p.fresh, l),
+                       __builtin_amdgcn_readlane(p.context, l), (uint64_t)readlane_d(p.at, l));
+    }
+    __syncthreads();
+    if (has) {
+        double at = p.at;
+        for (int r = p.r0; r < p.r1; r++) {
+            const int t0 = a.offsets[r], fresh = max(0, a.offsets[r + 1] - t0), context = a.context[r];
+            const double size = ka_size(a, fresh, context, rows);
+            if (d < at + size) {
+                sh.item = ka_tile(a, rows, x, r, t0, fresh, context, (uint64_t)at);
+                break;
+            }
+            at += size;
+        }
+    }
+    __syncthreads();
+    return sh.item;
+}
+
+// A tile in scalar registers.
+__device__ static inline KaItem ka_uniform(KaItem m) {
+    auto u32 = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    auto u64 = [&](uint64_t v) { return (uint64_t)(unsigned)u32((int)v) | (uint64_t)(unsigned)u32((int)(v >> 32)) << 32; };
+    return KaItem{u32(m.r), u32(m.tile), u32(m.t0), u32(m.fresh), u32(m.context), u64(m.p), u64(m.e)};
 }
 
 // ---- the kernel ------------------------------------------------------------------------------
 
 typedef _Float16 ka_h2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x3 __attribute__((ext_vector_type(3)));
+typedef u32x3 u32x3_any __attribute__((aligned(1)));
 
 // Eight codes and their scale to eight halves.
 __device__ static inline a16_h8 ka_halves(unsigned codes, float scale) {
@@ -183,8 +211,7 @@ __device__ static inline a16_h8 ka_halves(unsigned codes, float scale) {
 struct KaRaw {
     u32x4 q0, q1;  // blocks j and 4 + j of the half (j = lane / 16)
     unsigned q2;   // the lane's eighth of block 8
-    u32x2 w0;      // the half's scale bytes, from byte 0 (first half) or 1 on: eight,
-    unsigned w1;   // and the next four
+    u32x3 w;       // twelve scale bytes, the half's among them
     unsigned on;   // all ones, or 0 where there is no such position
 };
 
@@ -209,7 +236,6 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
     __shared__ __align__(8) float cr[ROWS], rl[ROWS], rm[ROWS];
     __shared__ __align__(8) unsigned char moved[KA_WAVES];
     __shared__ KaShared sh;
-    __shared__ KaItem item;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kh = w >> 2, pg = w & 3;
     const int kv = a.c.kv, rope = a.c.rope, nb = a.c.blocks, shift = a.c.shift;
     const KaPlan plan = ka_plan(a, ROWS, sh);
@@ -218,10 +244,7 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
     if (threadIdx.x == 0) a.cuts[blockIdx.x].k = 0;
 
     for (uint64_t at = x0; at < x1;) {
-        __syncthreads();
-        ka_find(a, plan, ROWS, at, &item);
-        __syncthreads();
-        const KaItem m = item;
+        const KaItem m = ka_uniform(ka_find(a, plan, ROWS, at, sh));
         at = m.e;
         const int rows = m.fresh * a.H, row0 = m.tile * ROWS, nr = min(ROWS, rows - row0);
         const int first = m.context - m.fresh;  // the position of the request's first token
@@ -232,6 +255,7 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
         const uint64_t head = units > 0 ? m.p + KA_LEAD : m.p, tail = units > 0 ? min(m.p + KA_LEAD + units, m.e) - 1 : m.p;
         const bool ends = x0 <= tail && tail < x1, whole = ends && x0 <= head;
         if (units > 0 ? u0 == u1 : !whole) continue;
+        __syncthreads();  // (what the tile before left in shared memory is read)
         const int s0 = KA_P * u0, s1 = min(end, KA_P * u1), nt = u1 - u0;
         const int slot = 2 * blockIdx.x + (m.p > x0 ? 1 : 0);  // of a partial result: the block's first tile, or its last
         const int32_t *table = a.table + (size_t)m.r * a.max_pages;
@@ -239,11 +263,12 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
         // The lane's blocks of its half, and which of the half's bytes are their scales. A block past the
         // row's last reads codes of another at scale 0.
         const int b0 = KA_HALF * kh + lg, b1 = b0 + 4, b2 = KA_HALF * kh + 8;
-        const unsigned none = 0x0c0c0c0cu, sel0 = b0 < nb ? 0x0c0c0c00u + kh + lg : none, sel1 = b1 < nb ? 0x0c0c0c00u + kh + lg : none,
-                       sel2 = b2 < nb ? 0x0c0c0c00u + kh : none;
+        // (twelve bytes from `from` on, which the row has: it ends 16 bytes past its codes, 32 where it has over 16 blocks)
+        const int from = kh == 0 ? 0 : nb > 16 ? KA_HALF : 4, w0 = KA_HALF * kh - from + lg;
+        const unsigned none = 0x0c0c0c0cu, sel0 = b0 < nb ? 0x0c0c0c00u + w0 : none, sel1 = b1 < nb ? 0x0c0c0c00u + w0 : none,
+                       sel2 = b2 < nb ? 0x0c0c0c00u + w0 - lg : none;
         const int at0 = b0 < nb ? 16 * b0 : 0, at1 = b1 < nb ? 16 * b1 : 0, at2 = b2 < nb ? 16 * b2 + 4 * lg : 0;
-        // (a row ends 16 bytes past its codes, 32 where it has over 16 blocks)
-        const int ats = 16 * nb + (KA_HALF * kh < nb ? 8 * kh : 0), atw = 16 * nb + (kh == 0 ? 8 : nb > 16 ? 16 : 0);
+        const int ats = 16 * nb + from;
         const bool v0 = 32 * b0 < kv, v1 = 32 * b1 < kv, v2 = 32 * b2 < kv;  // blocks of the entry, not of the rope part
 
         // the lane's position of tile j: its page, as the table has it (nothing looks at it before fetch(),
@@ -257,50 +282,54 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
             x.q0 = *gbl((const u32x4 *)(row + at0));
             x.q1 = *gbl((const u32x4 *)(row + at1));
             x.q2 = *gbl((const unsigned *)(row + at2));
-            x.w0 = *gbl((const u32x2 *)(row + ats));
-            x.w1 = *gbl((const unsigned *)(row + atw));
+            x.w = *(const GM_GLOBAL u32x3_any *)(row + ats);
         };
-        int page = -1;
-        KaRaw raw;
-        if (nt > 0) {
-            fetch(raw, 0, page_of(0));
-            if (nt > 1) page = page_of(1);
-        }
-
-        // the queries: wave w stages rows RPW w .. as operand rows of halves, scaled by 2^-e
+        // the first pages, then the queries, then the first codes, so that they are under way together
+        int page0 = -1, page = -1;
+        if (nt > 0) page0 = page_of(0);
+        if (nt > 1) page = page_of(1);
         _Float16 *stage = val[0];
         const int plane = ka_tid() & 63;
         float lsum[RPW], top[RPW];  // a row's sum, and its reference + KA_SLACK (of base 2)
         int eq[RPW], last[RPW];
         bool on[RPW];
+        // wave w stages rows RPW w .. as operand rows of halves, scaled by 2^-e
+        float v[RPW][KV4_BLOCKS_MAX / 2];
 #pragma unroll
         for (int i = 0; i < RPW; i++) {
-            const int r = RPW * w + i, g = row0 + min(r, nr - 1), t = g / a.H, h = g - t * a.H;
+            const int g = row0 + min(RPW * w + i, nr - 1), t = g / a.H, h = g - t * a.H;
             const float *qa = a.q_abs + (m.t0 + t) * a.ld_q_abs + (int64_t)h * kv, *qp = a.q_pe + (m.t0 + t) * a.ld_q_pe + (int64_t)h * rope;
-            float v[KV4_BLOCKS_MAX / 2];
-            float mx = 0.0f;
 #pragma unroll
             for (int k = 0; k < KV4_BLOCKS_MAX / 2; k++) {
                 const int col = 64 * k + plane;
-                v[k] = col < kv ? qa[col] : col - kv < rope ? qp[col - kv] : 0.0f;
-                mx = fmaxf(mx, fabsf(v[k]));
+                v[i][k] = 0.0f;
+                if (col < kv) v[i][k] = *gbl(qa + col);
+                else if (col - kv < rope) v[i][k] = *gbl(qp + col - kv);
             }
-            mx = wave_max_dpp_f(mx);
-            const int e = mx < INFINITY ? spl_exp(mx) : 0;
-            _Float16 *hi = stage + (16 * (r >> 3) + 4 * ((r & 7) >> 1) + (r & 1)) * KA_QROW, *lo = hi + 2 * KA_QROW;
-#pragma unroll
-            for (int k = 0; k < KV4_BLOCKS_MAX / 2; k++) {
-                _Float16 x, y;
-                spl_split(ldexpf(v[k], -e), x, y);
-                hi[64 * k + plane] = x;
-                lo[64 * k + plane] = y;
-            }
-            eq[i] = e;
             last[i] = min(first + t, s1 - 1);
             lsum[i] = 0.0f;
             top[i] = -INFINITY;
         }
-        __syncthreads();
+        KaRaw raw;
+        if (nt > 0) fetch(raw, 0, page0);
+#pragma unroll
+        for (int i = 0; i < RPW; i++) {
+            const int r = RPW * w + i;
+            float mx = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KV4_BLOCKS_MAX / 2; k++) mx = fmaxf(mx, fabsf(v[i][k]));
+            mx = wave_max_dpp_f(mx);
+            eq[i] = mx < INFINITY ? spl_exp(mx) : 0;
+            _Float16 *hi = stage + (16 * (r >> 3) + 4 * ((r & 7) >> 1) + (r & 1)) * KA_QROW, *lo = hi + 2 * KA_QROW;
+#pragma unroll
+            for (int k = 0; k < KV4_BLOCKS_MAX / 2; k++) {
+                _Float16 x, y;
+                spl_split(ldexpf(v[i][k], -eq[i]), x, y);
+                hi[64 * k + plane] = x;
+                lo[64 * k + plane] = y;
+            }
+        }
+        block_barrier();
         a16_h8 q[KA_HALF][MT];  // steps 0..3: eighths of blocks j; 4..7: of blocks 4 + j; 8: block 8
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
@@ -317,7 +346,7 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
         for (int c = 0; c < 4; c++)
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) acc[c][mt] = (aq_f4){0.0f, 0.0f, 0.0f, 0.0f};
-        __syncthreads();  // the staged queries are read; values may come
+        block_barrier();  // the staged queries are read; values may come
 
         // where the lane writes values (pieces 4 b0 .. + 3, then b1's 16 on, and its eighth of block 2) and scores
         const int mix = (2 * (l16 & 7)) ^ (l16 >> 2 & 1);
@@ -328,8 +357,8 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
         const int sat = (16 * pg + l16) * KA_SROW + ((2 * lg) ^ (l16 & 8) >> 1 ^ (pg & 1) << 1);
         // tile j's scores (this half's part) from `raw`, its values to shared memory
         auto scores = [&](int j) {
-            unsigned e0 = __builtin_amdgcn_perm(raw.w0[1], raw.w0[0], sel0) & raw.on, e1 = __builtin_amdgcn_perm(raw.w1, raw.w0[1], sel1) & raw.on,
-                     e2 = __builtin_amdgcn_perm(0u, raw.w1, sel2) & raw.on;
+            unsigned e0 = __builtin_amdgcn_perm(raw.w[1], raw.w[0], sel0) & raw.on, e1 = __builtin_amdgcn_perm(raw.w[2], raw.w[1], sel1) & raw.on,
+                     e2 = __builtin_amdgcn_perm(0u, raw.w[2], sel2) & raw.on;
             unsigned long long spoilt = __ballot(max(max(e0, e1), e2) == KV4_BYTE_NAN);
             if (spoilt) {  // such a block's values count as zeros, and its position's scores as NaN
                 if (e0 == KV4_BYTE_NAN) e0 = 0;
@@ -344,17 +373,17 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) d[mt] = (aq_f4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int g = 0; g < 2; g++) {
-                a16_h8 x[4];
+            for (int g = 0; g < 4; g++) {  // two eighths at a time
+                a16_h8 x[2];
 #pragma unroll
-                for (int k = 0; k < 4; k++) x[k] = ka_halves(g ? raw.q1[k] : raw.q0[k], g ? f1 : f0);
-                if (g ? v1 : v0)
+                for (int k = 0; k < 2; k++) x[k] = ka_halves(g < 2 ? raw.q0[2 * g + k] : raw.q1[2 * (g - 2) + k], g < 2 ? f0 : f1);
+                if (g < 2 ? v0 : v1)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) *(a16_h8 *)(dst + wat[k] + 128 * g) = x[k];
+                    for (int k = 0; k < 2; k++) *(a16_h8 *)(dst + wat[2 * (g & 1) + k] + 128 * (g >> 1)) = x[k];
 #pragma unroll
-                for (int k = 0; k < 4; k++)
+                for (int k = 0; k < 2; k++)
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++) d[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[4 * g + k][mt], x[k], d[mt], 0, 0, 0);
+                    for (int mt = 0; mt < MT; mt++) d[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[2 * g + k][mt], x[k], d[mt], 0, 0, 0);
             }
             const a16_h8 x = ka_halves(raw.q2, f2);
             if (v2) *(a16_h8 *)(dst + wat2) = x;
@@ -365,7 +394,7 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
             for (int mt = 0; mt < MT; mt++) t[mt] = make_float2(d[mt][0] + d[mt][2], d[mt][1] + d[mt][3]);
             if (spoilt || !__all(raw.on)) {
                 const float odd = !raw.on ? -INFINITY : __uint_as_float(0x7fc00000u);
-                if (!raw.on || (spoilt >> l16 & 1))
+                if (!raw.on || ((unsigned)spoilt >> l16 & 1))
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) t[mt] = make_float2(odd, odd);
             }
@@ -373,25 +402,26 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
             for (int mt = 0; mt < MT; mt++) *(float2 *)&sc[j & 1][kh][sat + 8 * mt] = t[mt];
         };
         // tile j's exponentials from its scores
-        int rat[RPW];          // the lane's position's score of its rows
-        _Float16 *pat[RPW];    // the operand that the lane writes: its pair of positions' first parts, or the second
-        {
-            const int op = 32 * (lane >> 5) + 8 * ((lane & 15) >> 2) + 4 * ((lane & 31) >> 4) + (lane & 2);  // the pair's operand slot
-#pragma unroll
-            for (int i = 0; i < RPW; i++) {
-                const int r = RPW * w + i, o = 16 * (r >> 3) + 4 * ((r & 7) >> 1) + (r & 1) + 2 * (lane & 1);
-                rat[i] = lane * KA_SROW + (r ^ (lane & 8) >> 1 ^ (lane & 16) >> 3);
-                pat[i] = pr + o * KA_PROW + (op ^ 8 * ((o & 7) ^ (o >> 3 & 1)));
-            }
-        }
+        // where the lane finds its position's scores and puts its pair of positions' first parts, or the second,
+        // but for the row
+        const int rat = lane * KA_SROW, rmix = (lane & 8) >> 1 ^ (lane & 16) >> 3;
+        const int pat = (32 * (lane >> 5) + 8 * ((lane & 15) >> 2) + 4 * ((lane & 31) >> 4) + (lane & 2)) ^ 16 * (lane & 1), podd = 2 * KA_PROW * (lane & 1);
         const unsigned pick = lane & 1 ? 0x03020706u : 0x05040100u;  // of (the partner's, the lane's) pair of parts
         auto softmax = [&](int j) {
             const int s = s0 + KA_P * j + lane;
             float t[RPW];
             bool up[RPW], any = false;
+            float xa[RPW], xb[RPW];
 #pragma unroll
             for (int i = 0; i < RPW; i++) {
-                const float x = sc[j & 1][0][rat[i]] + sc[j & 1][1][rat[i]];
+                const int at = rat + ((RPW * w + i) ^ rmix);
+                xa[i] = sc[j & 1][0][at];
+                xb[i] = sc[j & 1][1][at];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < RPW; i++) {
+                const float x = xa[i] + xb[i];
                 t[i] = ldexpf(x, eq[i]);
                 on[i] = s <= last[i] && x != -INFINITY;
                 up[i] = on[i] && t[i] * scale > top[i];
@@ -423,7 +453,8 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
                 both.x = (_Float16)e;
                 both.y = (_Float16)fmaf((float)both.x, -1.0f, e);
                 const unsigned me = __builtin_bit_cast(unsigned, both), other = (unsigned)__builtin_amdgcn_update_dpp(0, (int)me, DPP_QUAD_1032, 0xF, 0xF, false);
-                *(unsigned *)pat[i] = __builtin_amdgcn_perm(other, me, pick);
+                const int r = RPW * w + i, o = 16 * (r >> 3) + 4 * ((r & 7) >> 1) + (r & 1);  // (the second part's row is o + 2)
+                *(unsigned *)&pr[o * KA_PROW + podd + (pat ^ 8 * ((o & 7) ^ (o >> 3 & 1)))] = __builtin_amdgcn_perm(other, me, pick);
             }
         };
         // where the lane reads exponentials, and four rows' values of each 16 columns
@@ -437,6 +468,18 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
         // tile j's values weighted
         auto values = [&](int j) {
             const u32x2 mv = *(const u32x2 *)moved;
+            const _Float16 *src = val[j & 1];
+            a16_h8 p[MT], v[4];
+            auto load = [&](int ks) {
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) p[mt] = *(const a16_h8 *)(pr + 16 * mt * KA_PROW + (ks ? pin ^ 32 : pin));
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const a16_h4 x = a16_tr(src + vin[c] + 32 * ks * KA_VROW), y = a16_tr(src + vin[c] + (32 * ks + 16) * KA_VROW);
+                    v[c] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+                }
+            };
+            load(0);
             if (__builtin_amdgcn_readfirstlane(mv[0] | mv[1])) {
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++) {
@@ -445,19 +488,13 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
                     for (int c = 0; c < 4; c++) acc[c][mt] *= (aq_f4){f.x, f.y, f.x, f.y};
                 }
             }
-            const _Float16 *src = val[j & 1];
 #pragma unroll
             for (int ks = 0; ks < KA_P / 32; ks++) {
-                a16_h8 p[MT];
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++) p[mt] = *(const a16_h8 *)(pr + 16 * mt * KA_PROW + (ks ? pin ^ 32 : pin));
+                for (int c = 0; c < 4; c++)
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const a16_h4 x = a16_tr(src + vin[c] + 32 * ks * KA_VROW), y = a16_tr(src + vin[c] + (32 * ks + 16) * KA_VROW);
-                    const a16_h8 v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++) acc[c][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[mt], v, acc[c][mt], 0, 0, 0);
-                }
+                    for (int mt = 0; mt < MT; mt++) acc[c][mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[mt], v[c], acc[c][mt], 0, 0, 0);
+                if (ks + 1 < KA_P / 32) load(ks + 1);
             }
         };
         const bool mine = 64 * w < kv;  // the wave has columns
