@@ -159,7 +159,7 @@ __device__ __attribute__((always_inline)) static void gemv_run(GemvArgs a, int b
         const int8_t *q = a.q;
         const float *s = a.s;
         float *y = a.y;
-        if (MODE == GV_PLAIN && r >= a.rows) {  // the second matrix (whole row groups)
+        if (MODE == GV_PLAIN && a.rows_b && r >= a.rows) {  // the second matrix (whole row groups)
             r -= a.rows;
             n = a.rows_b;
             q = a.qb;
