@@ -29,6 +29,7 @@
 #include <vector>
 
 #include "gmoe_model.h"
+#include "gmoe_serve.h"
 #include "common.h"
 #include "dense.h"
 #include "attn.h"
@@ -108,6 +109,16 @@ struct gmoe_model {
     int *xe = nullptr;
     __half *zeros = nullptr;
     std::vector<void *> allocs;  // every device allocation, freed by gmoe_model_destroy
+    // several requests (gmoe_model_step): each request's positions, the pages left, and on the device
+    // the pool of every attention layer, the tables, a step's arrays and its rows' logits
+    std::vector<int> seen;
+    int page_size = 0, n_pages = 0, width = 0, n_free = 0;
+    uint8_t *pages = nullptr;
+    int32_t *table = nullptr, *free_pages = nullptr, *step_in = nullptr, *step_maps = nullptr;
+    float *new_comp = nullptr, *new_pe = nullptr, *rows_x = nullptr, *rows_logits = nullptr, *rows_out = nullptr;
+    uint8_t *attend_work = nullptr, *score_work = nullptr;
+    size_t attend_bytes = 0, score_bytes = 0;
+    int rows_max = 0;  // rows of one LM head call
 };
 
 namespace {
@@ -530,11 +541,11 @@ void gemm_launch(gmoe_model *m, const int8_t *q, const float *s, const int8_t *q
     else gemm_tiles<32, 1>(a, mode, panels, st);
 }
 
-int attention_batch(gmoe_model *m, int l, int pos0, int n, hipStream_t st) {
+// The products of n tokens of x before the attention: q_a, kv_a and the full queries.
+void attn_queries(gmoe_model *m, const AttnDev &A, int n, hipStream_t st) {
     const gmoe_model_config &c = m->c;
-    const AttnDev &A = m->attn[l];
     const int gs = c.group_size, H = c.n_heads, kv = c.kv_lora_rank, rope = c.rope_dim, D = c.dim;
-    const int ql = c.q_lora_rank, hk = c.head_k_dim, vh = c.v_head_dim;
+    const int ql = c.q_lora_rank, hk = c.head_k_dim;
     if (gemm_batch(m, n)) {
         gemm_inputs(m, m->x, D, D, A.attn_norm, n, st);
         // q_a and kv_a, two small products of the same inputs, in one launch
@@ -550,32 +561,38 @@ int attention_batch(gmoe_model *m, int l, int pos0, int n, hipStream_t st) {
         launch_gemv(qa, GV_PLAIN, st, n);
         launch_gemv(batched(gemv(A.q_b_q, A.q_b_s, m->q_a, A.q_a_norm, m->q_full, H * hk, ql, gs), ql, H * hk), GV_PLAIN, st, n);
     }
-    const AttnArgs aa = attn_args(m, l, pos0);
-    GemvArgs kb = batched(gemv(A.k_b_q, A.k_b_s, m->q_full, nullptr, m->q_abs, H * kv, c.qk_nope_dim, gs), H * hk, H * kv);
+}
+
+// The absorbed queries of n tokens, group h: k_b_h . q_nope_h, as one GEMM ...
+void attn_absorb_gemm(gmoe_model *m, const AttnDev &A, int n, hipStream_t st) {
+    const gmoe_model_config &c = m->c;
+    const int H = c.n_heads, kv = c.kv_lora_rank, hk = c.head_k_dim;
+    gemm_inputs(m, m->q_full, H * hk, H * hk, nullptr, n, st);
+    gemm_launch(m, A.k_b_q, A.k_b_s, nullptr, nullptr, H * kv, c.qk_nope_dim, kv, hk, H * hk, m->q_abs, H * kv, nullptr, 0,
+                QG_PLAIN, n, st);
+}
+
+// ... or as the batched matrix-vector product that k_attn_query takes.
+GemvArgs attn_absorb_gemv(gmoe_model *m, const AttnDev &A) {
+    const gmoe_model_config &c = m->c;
+    const int H = c.n_heads, kv = c.kv_lora_rank, hk = c.head_k_dim;
+    GemvArgs kb = batched(gemv(A.k_b_q, A.k_b_s, m->q_full, nullptr, m->q_abs, H * kv, c.qk_nope_dim, c.group_size), H * hk, H * kv);
     kb.x_rows = kv;
     kb.x_stride = hk;
+    return kb;
+}
+
+// The products after the attention, per head concat_h = v_b_h . ctx_h, then x += attn_out . concat.
+void attn_outputs(gmoe_model *m, const AttnDev &A, int n, hipStream_t st) {
+    const gmoe_model_config &c = m->c;
+    const int gs = c.group_size, H = c.n_heads, kv = c.kv_lora_rank, D = c.dim, vh = c.v_head_dim;
     if (gemm_batch(m, n)) {
-        // the absorbed queries as one GEMM (group h: k_b_h . q_nope_h), then the cache entries
-        // and rotated queries (k_attn_query's last block alone)
-        gemm_inputs(m, m->q_full, H * hk, H * hk, nullptr, n, st);
-        gemm_launch(m, A.k_b_q, A.k_b_s, nullptr, nullptr, H * kv, c.qk_nope_dim, kv, hk, H * hk, m->q_abs, H * kv,
-                    nullptr, 0, QG_PLAIN, n, st);
-        launch_prep(kb, aa, st, n);
-    } else {
-        launch_query(kb, aa, st, n);  // every token's cache entry before any token's attention
-    }
-    if (attn_tile_ok(c))
-        launch_attn_tile(m, aa, n, st);
-    else
-        launch_attn_cache_batch(m, aa, n, st);
-    if (gemm_batch(m, n)) {
-        // per head: concat_h = v_b_h . ctx_h, then x += attn_out . concat
         gemm_inputs(m, m->ctx, H * kv, H * kv, nullptr, n, st);
         gemm_launch(m, A.v_b_q, A.v_b_s, nullptr, nullptr, H * vh, kv, vh, kv, H * kv, m->concat, H * vh, nullptr, 0,
                     QG_PLAIN, n, st);
         gemm_inputs(m, m->concat, H * vh, H * vh, nullptr, n, st);
         gemm_launch(m, A.out_q, A.out_s, nullptr, nullptr, D, H * vh, D, 0, H * vh, m->x, D, m->x, D, QG_RESID, n, st);
-        return GMOE_OK;
+        return;
     }
     GemvArgs vb = batched(gemv(A.v_b_q, A.v_b_s, m->ctx, nullptr, m->concat, H * vh, kv, gs), H * kv, H * vh);
     vb.x_rows = vh;
@@ -585,6 +602,25 @@ int attention_batch(gmoe_model *m, int l, int pos0, int n, hipStream_t st) {
     ao.resid = m->x;
     ao.br = D;
     launch_gemv(ao, GV_RESID, st, n);
+}
+
+int attention_batch(gmoe_model *m, int l, int pos0, int n, hipStream_t st) {
+    const AttnDev &A = m->attn[l];
+    attn_queries(m, A, n, st);
+    const AttnArgs aa = attn_args(m, l, pos0);
+    const GemvArgs kb = attn_absorb_gemv(m, A);
+    if (gemm_batch(m, n)) {
+        // the absorbed queries, then the cache entries and rotated queries (k_attn_query's last block alone)
+        attn_absorb_gemm(m, A, n, st);
+        launch_prep(kb, aa, st, n);
+    } else {
+        launch_query(kb, aa, st, n);  // every token's cache entry before any token's attention
+    }
+    if (attn_tile_ok(m->c))
+        launch_attn_tile(m, aa, n, st);
+    else
+        launch_attn_cache_batch(m, aa, n, st);
+    attn_outputs(m, A, n, st);
     return GMOE_OK;
 }
 
@@ -984,5 +1020,295 @@ extern "C" int gmoe_model_read_cache(gmoe_model *m, int layer, int pos0, int n, 
     if (pe_out)
         MH_OK(hipMemcpyAsync(pe_out, m->pe + row0 * rope, (size_t)n * rope * sizeof(float), hipMemcpyDeviceToHost, st));
     MH_OK(hipStreamSynchronize(st));
+    return GMOE_OK;
+}
+
+// ---- several requests at once (gmoe_serve.h's operators on the whole model) --------------------
+
+namespace {
+
+constexpr int kStepRows = 64;  // rows of one LM head call: 40 MB of logits at GLM-4.7-Flash's vocabulary
+
+// Token blockIdx.x of a step: its cache entry (the normalised kv, the rotated rope part) and its
+// heads' rotated queries, with attn_prep_run's operations (infer.c:1000-1016) at the token's own
+// position; a token without one (-1) is turned as at 0, and no one reads it.
+__global__ __launch_bounds__(DM_BLOCK) void k_step_prep(const float *__restrict__ kv_a, const float *__restrict__ kv_norm,
+                                                        const float *__restrict__ q_full, const float *__restrict__ rope_cs,
+                                                        const int32_t *__restrict__ position, int H, int kv, int rope, int head_k,
+                                                        int nope, float *__restrict__ comp, float *__restrict__ pe, float *__restrict__ q_pe) {
+    __shared__ double red[DM_BLOCK / 64];
+    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    kv_a += (size_t)t * (kv + rope);
+    q_full += (size_t)t * H * head_k;
+    comp += (size_t)t * kv;
+    pe += (size_t)t * rope;
+    q_pe += (size_t)t * H * rope;
+    double ss = 0.0;
+    for (int i = tid; i < kv; i += DM_BLOCK) ss += (double)kv_a[i] * (double)kv_a[i];
+    ss = wave_sum_dpp(ss);
+    if (lane == 0) red[w] = ss;
+    __syncthreads();
+    ss = (red[0] + red[1]) + (red[2] + red[3]);
+    const float mean = (float)(ss / (double)kv);
+    const float inv = __fdiv_rn(1.0f, sqrt_rn_f32(__fadd_rn(mean, 1e-5f)));
+    for (int i = tid; i < kv; i += DM_BLOCK) comp[i] = __fmul_rn(__fmul_rn(kv_a[i], inv), kv_norm[i]);
+    const float *cs = rope_cs + (size_t)max(position[t], 0) * rope;  // rope / 2 pairs of (cos, sin)
+    const int half = rope >> 1;
+    for (int j = tid; j < (H + 1) * half; j += DM_BLOCK) {
+        const int h = j / half - 1, i = j % half;
+        const float *src = h < 0 ? kv_a + kv : q_full + (size_t)h * head_k + nope;
+        float *dst = h < 0 ? pe : q_pe + (size_t)h * rope;
+        const float c = cs[2 * i], s = cs[2 * i + 1], v0 = src[2 * i], v1 = src[2 * i + 1];
+        dst[2 * i] = __fsub_rn(__fmul_rn(v0, c), __fmul_rn(v1, s));
+        dst[2 * i + 1] = __fadd_rn(__fmul_rn(v0, s), __fmul_rn(v1, c));
+    }
+}
+
+// Row blockIdx.y of a step's rows: token rows[blockIdx.y]'s x.
+__global__ __launch_bounds__(DM_BLOCK) void k_step_rows(const float *__restrict__ x, const int32_t *__restrict__ rows, int dim,
+                                                        float *__restrict__ out) {
+    const int i = blockIdx.x * DM_BLOCK + threadIdx.x;
+    if (i < dim) out[(size_t)blockIdx.y * dim + i] = x[(size_t)rows[blockIdx.y] * dim + i];
+}
+
+// A request's n pages behind the pool's n_free.
+__global__ __launch_bounds__(DM_BLOCK) void k_step_release(const int32_t *__restrict__ table, int n, int32_t *__restrict__ free_pages,
+                                                           int n_free) {
+    const int i = blockIdx.x * DM_BLOCK + threadIdx.x;
+    if (i < n) free_pages[n_free + i] = table[i];
+}
+
+// Layer l's attention of a step of n tokens: products as a prefill's, the rows into the paged cache
+// and the attention over it.
+int attention_step(gmoe_model *m, int l, int n, const gmoe_batch *b, hipStream_t st) {
+    const gmoe_model_config &c = m->c;
+    const AttnDev &A = m->attn[l];
+    const int H = c.n_heads, kv = c.kv_lora_rank, rope = c.rope_dim;
+    attn_queries(m, A, n, st);
+    if (gemm_batch(m, n)) attn_absorb_gemm(m, A, n, st);
+    else launch_gemv(attn_absorb_gemv(m, A), GV_PLAIN, st, n);
+    hipLaunchKernelGGL(k_step_prep, dim3((unsigned)n), dim3(DM_BLOCK), 0, st, m->kv_a, A.kv_a_norm, m->q_full, m->rope_cs, b->position, H,
+                       kv, rope, c.head_k_dim, c.qk_nope_dim, m->new_comp, m->new_pe, m->q_pe);
+    const size_t pool = (size_t)m->n_pages * m->page_size * gmoe_kv4_row_bytes(kv, rope);
+    const gmoe_kv4 cache = {m->pages + (size_t)l * pool, kv, rope, m->n_pages, m->page_size};
+    if (int rc = gmoe_kv4_append(m->device, &cache, n, m->new_comp, kv, m->new_pe, rope, b->slot, st)) return rc;
+    const gmoe_kv4_heads h = {H, 1.0f / sqrtf((float)c.head_k_dim), m->q_abs, (int64_t)H * kv, m->q_pe, (int64_t)H * rope,
+                              m->ctx, (int64_t)H * kv, m->attend_work, m->attend_bytes};
+    if (int rc = gmoe_kv4_attend(m->device, &cache, b, &h, st)) return rc;
+    attn_outputs(m, A, n, st);
+    return GMOE_OK;
+}
+
+// The launches of a step: `in` holds its arrays in step_in's order, nr rows.
+int step_run(gmoe_model *m, const gmoe_model_batch *b, int n, size_t nr, const std::vector<int32_t> &in, hipStream_t st) {
+    const gmoe_model_config &c = m->c;
+    const int R = b->n_requests, V = c.vocab_size, D = c.dim;
+    MH_OK(hipMemcpyAsync(m->step_in, in.data(), in.size() * sizeof(int32_t), hipMemcpyHostToDevice, st));
+    const int32_t *tokens = m->step_in + 2 * R + 1, *row_at = tokens + n, *given = row_at + nr;
+    gmoe_batch g{};
+    g.n_requests = R;
+    g.max_tokens = n;
+    g.max_pages = m->width;
+    g.page_size = m->page_size;
+    g.seen = m->step_in;
+    g.fresh = m->step_in + R;
+    g.n_free = m->step_in + 2 * R;
+    g.free_pages = m->free_pages;
+    g.table = m->table;
+    g.offsets = m->step_maps;
+    g.context = g.offsets + R + 1;
+    g.request = g.context + R;
+    g.position = g.request + n;
+    g.slot = g.position + n;
+    g.totals = g.slot + n;
+    if (int rc = gmoe_page_maps(m->device, &g, st)) return rc;
+    hipLaunchKernelGGL(k_embed_batch, dim3((unsigned)((D + DM_BLOCK - 1) / DM_BLOCK), (unsigned)n), dim3(DM_BLOCK), 0, st, m->tok_q,
+                       m->tok_s, tokens, V, D, c.group_size, m->x);
+    // the model forms of infer.c:1817-1881 that have attention; one token's MoE layers as forward_token's
+    const int n_run = c.attn_layers == c.n_layers ? c.n_layers : 1;
+    int rc = GMOE_OK, n_moe = 0, relay = 0, w = 0;
+    for (int l = 1; l < n_run; l++) {
+        if (!m->moe_on[l]) continue;
+        if (!gm_layer_ready(m->moe, l)) {
+            gm_set_err("gmoe_model_step: MoE layer %d is not uploaded to the model's context", l);
+            return GMOE_ERR_INVALID;
+        }
+        n_moe++;
+    }
+    if (n == 1 && n_moe > 0) rc = gm_decode_begin(m->moe, n_moe, st, &relay);
+    for (int l = 0; l < n_run && !rc; l++) {
+        rc = attention_step(m, l, n, &g, st);
+        if (!rc && l == 0 && c.has_l0_ffn) rc = n == 1 ? dense_ffn(m, st) : dense_ffn_batch(m, n, st);
+        if (!rc && l > 0 && m->moe_on[l])
+            rc = relay ? gm_decode_layer(m->moe, l, w++, m->x, m->x, m->moe_flags, st)
+                       : gmoe_forward(m->moe, l, n, m->x, m->x, m->moe_flags, st);
+    }
+    if (rc) {
+        if (relay) gm_decode_abort(m->moe);
+        return rc;
+    }
+    float *lp = m->rows_out, *ent = lp + m->rows_max, *tlp = ent + m->rows_max;
+    int32_t *tid = (int32_t *)(tlp + (size_t)m->rows_max * GMOE_TOP_MAX);
+    const size_t T = (size_t)b->top;
+    const bool score = b->given || b->entropy || T > 0;
+    for (size_t at = 0; at < nr && (score || b->logits); at += m->rows_max) {
+        const int k = (int)std::min<size_t>(m->rows_max, nr - at);
+        hipLaunchKernelGGL(k_step_rows, dim3((unsigned)((D + DM_BLOCK - 1) / DM_BLOCK), (unsigned)k), dim3(DM_BLOCK), 0, st, m->x,
+                           row_at + at, D, m->rows_x);
+        if (gemm_batch(m, k)) {
+            gemm_inputs(m, m->rows_x, D, D, m->output_norm, k, st);
+            gemm_launch(m, m->out_q, m->out_s, nullptr, nullptr, V, D, V, 0, D, m->rows_logits, V, nullptr, 0, QG_PLAIN, k, st);
+        } else {
+            launch_gemv(batched(gemv(m->out_q, m->out_s, m->rows_x, m->output_norm, m->rows_logits, V, D, c.group_size), D, V), GV_PLAIN, st,
+                        k);
+        }
+        MH_OK(hipGetLastError());
+        if (score) {
+            const gmoe_logprobs_args a = {k, V, b->given ? 1 : 0, b->top, m->rows_logits, V, given + at, lp, b->entropy ? ent : nullptr,
+                                          tid, tlp, m->score_work, m->score_bytes};
+            if (int e = gmoe_logprobs(m->device, &a, st)) return e;
+            if (b->given) MH_OK(hipMemcpyAsync(b->logprob + at, lp, k * sizeof(float), hipMemcpyDeviceToHost, st));
+            if (b->entropy) MH_OK(hipMemcpyAsync(b->entropy + at, ent, k * sizeof(float), hipMemcpyDeviceToHost, st));
+            if (T) MH_OK(hipMemcpyAsync(b->top_id + at * T, tid, k * T * sizeof(int32_t), hipMemcpyDeviceToHost, st));
+            if (T) MH_OK(hipMemcpyAsync(b->top_logprob + at * T, tlp, k * T * sizeof(float), hipMemcpyDeviceToHost, st));
+        }
+        if (b->logits)
+            MH_OK(hipMemcpyAsync(b->logits + at * V, m->rows_logits, (size_t)k * V * sizeof(float), hipMemcpyDeviceToHost, st));
+    }
+    MH_OK(hipGetLastError());
+    return GMOE_OK;
+}
+
+}  // namespace
+
+extern "C" int gmoe_model_open_pages(gmoe_model *m, int max_requests, int page_size, int n_pages) {
+    if (!m) {
+        gm_set_err("gmoe_model_open_pages: null model");
+        return GMOE_ERR_INVALID;
+    }
+    const gmoe_model_config &c = m->c;
+    const size_t row = gmoe_kv4_row_bytes(c.kv_lora_rank, c.rope_dim);
+    if (m->page_size || c.attn_layers < 1 || !row || c.n_heads > 256 || max_requests < 1 || max_requests > GMOE_MAX_REQUESTS ||
+        page_size < 1 || page_size > 65536 || (page_size & (page_size - 1)) || n_pages < 1 || (long long)n_pages * page_size >= (1ll << 31)) {
+        gm_set_err("gmoe_model_open_pages: %d requests (1..%d), %d pages of %d positions (a power of two up to 65536, fewer than 2^31 in "
+                   "all), %d attention layers of ranks %d + %d and %d heads, %s",
+                   max_requests, GMOE_MAX_REQUESTS, n_pages, page_size, c.attn_layers, c.kv_lora_rank, c.rope_dim, c.n_heads,
+                   m->page_size ? "open already" : "not open");
+        return GMOE_ERR_INVALID;
+    }
+    MH_OK(hipSetDevice(m->device));
+    const size_t R = (size_t)max_requests, B = (size_t)std::max(1, c.max_batch), width = ((size_t)c.cache_cap + page_size - 1) / page_size;
+    m->rows_max = (int)std::min<size_t>(kStepRows, B);
+    for (int n = 1; n <= m->rows_max; n++) m->score_bytes = std::max(m->score_bytes, gmoe_logprobs_workspace(n, c.vocab_size, GMOE_TOP_MAX));
+    m->attend_bytes = gmoe_kv4_attend_workspace(c.n_heads, c.kv_lora_rank);
+    int rc = GMOE_OK;
+    rc |= mdalloc(m, &m->pages, (size_t)c.attn_layers * n_pages * page_size * row);
+    rc |= mdalloc(m, &m->table, R * width);
+    rc |= mdalloc(m, &m->free_pages, (size_t)n_pages);
+    rc |= mdalloc(m, &m->step_in, 2 * R + 1 + 3 * B);           // seen, fresh, pages left; tokens, rows, given
+    rc |= mdalloc(m, &m->step_maps, 2 * R + 1 + 3 * B + 3);     // offsets, context; request, position, slot; totals
+    rc |= mdalloc(m, &m->new_comp, B * c.kv_lora_rank);
+    rc |= mdalloc(m, &m->new_pe, B * c.rope_dim);
+    rc |= mdalloc(m, &m->rows_x, (size_t)m->rows_max * c.dim);
+    rc |= mdalloc(m, &m->rows_logits, (size_t)m->rows_max * c.vocab_size);
+    rc |= mdalloc(m, &m->rows_out, (size_t)m->rows_max * (2 + 2 * GMOE_TOP_MAX));
+    rc |= mdalloc(m, &m->attend_work, m->attend_bytes);
+    rc |= mdalloc(m, &m->score_work, m->score_bytes);
+    if (rc) return GMOE_ERR_NOMEM;  // (what was allocated goes with the model)
+    std::vector<int32_t> ids((size_t)n_pages);
+    for (int i = 0; i < n_pages; i++) ids[i] = n_pages - 1 - i;  // taken from the end: page 0 first
+    MH_OK(hipMemcpy(m->free_pages, ids.data(), ids.size() * sizeof(int32_t), hipMemcpyHostToDevice));
+    m->seen.assign(R, 0);
+    m->width = (int)width;
+    m->n_free = m->n_pages = n_pages;
+    m->page_size = page_size;
+    return GMOE_OK;
+}
+
+extern "C" int gmoe_model_free_pages(const gmoe_model *m) { return m && m->page_size ? m->n_free : -1; }
+
+extern "C" int gmoe_model_release(gmoe_model *m, int request, void *stream) {
+    if (!m || !m->page_size || request < 0 || request >= (int)m->seen.size()) {
+        gm_set_err("gmoe_model_release: request %d of %d", request, m ? (int)m->seen.size() : 0);
+        return GMOE_ERR_INVALID;
+    }
+    const int n = (m->seen[request] + m->page_size - 1) / m->page_size;
+    if (n == 0) return GMOE_OK;
+    MH_OK(hipSetDevice(m->device));
+    hipStream_t st = (hipStream_t)stream;
+    hipLaunchKernelGGL(k_step_release, dim3((unsigned)((n + DM_BLOCK - 1) / DM_BLOCK)), dim3(DM_BLOCK), 0, st,
+                       m->table + (size_t)request * m->width, n, m->free_pages, m->n_free);
+    MH_OK(hipGetLastError());
+    MH_OK(hipStreamSynchronize(st));
+    m->seen[request] = 0;
+    m->n_free += n;
+    return GMOE_OK;
+}
+
+extern "C" int gmoe_model_step(gmoe_model *m, const gmoe_model_batch *b, void *stream) {
+    if (!m || !b || !b->fresh || !b->tokens) {
+        gm_set_err("gmoe_model_step: null argument");
+        return GMOE_ERR_INVALID;
+    }
+    const gmoe_model_config &c = m->c;
+    const int R = b->n_requests, P = m->page_size, B = std::max(1, c.max_batch);
+    if (!P || R < 1 || R > (int)m->seen.size()) {
+        gm_set_err("gmoe_model_step: %d requests outside 1..%d (gmoe_model_open_pages)", R, (int)m->seen.size());
+        return GMOE_ERR_INVALID;
+    }
+    if (b->top < 0 || b->top > GMOE_TOP_MAX || (b->top > 0 && (!b->top_id || !b->top_logprob)) || (b->given && !b->logprob)) {
+        gm_set_err("gmoe_model_step: %d alternatives outside 0..%d, or no place for what is asked", b->top, GMOE_TOP_MAX);
+        return GMOE_ERR_INVALID;
+    }
+    if (!m->globals) {
+        gm_set_err("gmoe_model_step: gmoe_model_upload has not succeeded");
+        return GMOE_ERR_INVALID;
+    }
+    for (int l = 0; l < c.attn_layers; l++)
+        if (!m->attn[l].set) {
+            gm_set_err("gmoe_model_step: attention layer %d is not uploaded", l);
+            return GMOE_ERR_INVALID;
+        }
+    // the step's tokens and rows, and the pages it takes
+    long long n = 0, pages = 0;
+    std::vector<int32_t> rows;
+    for (int r = 0; r < R; r++) {
+        const int fresh = b->fresh[r];
+        if (fresh < 0 || (long long)m->seen[r] + fresh > c.cache_cap) {
+            gm_set_err("gmoe_model_step: request %d: %d new tokens at position %d (cache_cap %d)", r, fresh, m->seen[r], c.cache_cap);
+            return GMOE_ERR_INVALID;
+        }
+        n += fresh;
+        pages += (m->seen[r] + fresh + P - 1) / P - (m->seen[r] + P - 1) / P;
+        if (n > B) break;
+        for (int i = b->every ? 0 : std::max(0, fresh - 1); i < fresh; i++) rows.push_back((int32_t)(n - fresh + i));
+    }
+    if (n < 1 || n > B) {
+        gm_set_err("gmoe_model_step: %lld tokens outside 1..%d (the model's max_batch)", n, B);
+        return GMOE_ERR_INVALID;
+    }
+    if (pages > m->n_free) {
+        gm_set_err("gmoe_model_step: %lld pages of %d positions are needed, %d are free", pages, P, m->n_free);
+        return GMOE_ERR_NOMEM;
+    }
+    MH_OK(hipSetDevice(m->device));
+    hipStream_t st = (hipStream_t)stream;
+    // one copy: seen, fresh, the pages left, the tokens, the rows' tokens, the given ids
+    std::vector<int32_t> in;
+    in.reserve(2 * (size_t)R + 1 + (size_t)n + 2 * rows.size());
+    in.insert(in.end(), m->seen.begin(), m->seen.begin() + R);
+    in.insert(in.end(), b->fresh, b->fresh + R);
+    in.push_back(m->n_free);
+    in.insert(in.end(), b->tokens, b->tokens + n);
+    in.insert(in.end(), rows.begin(), rows.end());
+    if (b->given) in.insert(in.end(), b->given, b->given + rows.size());
+    int rc = step_run(m, b, (int)n, rows.size(), in, st);
+    // also after an error: copies may still be under way from `in` and into b's arrays
+    const hipError_t done = hipStreamSynchronize(st);
+    if (!rc) MH_OK(done);
+    if (m->moe && gm_take_launch_error(m->moe) && !rc) rc = GMOE_ERR_HIP;
+    if (rc) return rc;
+    for (int r = 0; r < R; r++) m->seen[r] += b->fresh[r];
+    m->n_free -= (int)pages;
     return GMOE_OK;
 }

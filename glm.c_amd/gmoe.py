@@ -326,6 +326,11 @@ class ModelWeights(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in _MODEL_FIELDS]
 
 
+class ModelBatch(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_requests", "every", "top")] + \
+               [(n, C.c_void_p) for n in ("fresh", "tokens", "given", "logprob", "entropy", "top_id", "top_logprob", "logits")]
+
+
 # GLM-4.7-Flash's dense side (47 layers, MLA attention on every layer, dense layer 0)
 GLM47_FLASH_MODEL = dict(dim=2048, hidden_dim=10240, n_layers=47, n_heads=20, vocab_size=154880, q_lora_rank=768,
                          kv_lora_rank=512, rope_dim=64, qk_nope_dim=192, head_k_dim=256, v_head_dim=256, group_size=32)
@@ -394,8 +399,13 @@ class Model:
             self.lib.gmoe_model_set_moe.argtypes = [P, P, P, C.c_int]
             self.lib.gmoe_model_forward_token.argtypes = [P, C.c_int, C.c_int, C.c_int, P, P, P, P, P]
             self.lib.gmoe_model_prefill.argtypes = [P, P, C.c_int, C.c_int, P, P, P]
+            self.lib.gmoe_model_open_pages.argtypes = [P, C.c_int, C.c_int, C.c_int]
+            self.lib.gmoe_model_step.argtypes = [P, C.POINTER(ModelBatch), P]
+            self.lib.gmoe_model_release.argtypes = [P, C.c_int, P]
+            self.lib.gmoe_model_free_pages.argtypes = [P]
             for f in ("gmoe_model_create", "gmoe_model_upload", "gmoe_model_upload_attn", "gmoe_model_set_moe",
-                      "gmoe_model_forward_token", "gmoe_model_prefill"):
+                      "gmoe_model_forward_token", "gmoe_model_prefill", "gmoe_model_open_pages", "gmoe_model_step",
+                      "gmoe_model_release", "gmoe_model_free_pages"):
                 getattr(self.lib, f).restype = C.c_int
             self.lib.gmoe_model_destroy.argtypes = [P]
             self.lib.gmoe_model_destroy.restype = None
@@ -430,6 +440,37 @@ class Model:
         check(self.lib.gmoe_model_prefill(self.h, ptr(toks), int(toks.size), int(pos0), ptr(self.logits), None, stream),
               "gmoe_model_prefill")
         return self.logits
+
+    def open_pages(self, max_requests, page_size, n_pages):
+        """A paged latent cache in 4 bits for max_requests requests (gmoe_model_open_pages)."""
+        check(self.lib.gmoe_model_open_pages(self.h, max_requests, page_size, n_pages), "gmoe_model_open_pages")
+
+    def step(self, fresh, tokens, every=False, given=None, top=0, logits=False, stream=None):
+        """gmoe_model_step: new tokens of requests 0 .. len(fresh) - 1; a row a request that has any, or with
+        `every` a row a token. Returns {"entropy", "logprob" (given), "top_id", "top_logprob", "logits"}."""
+        fresh = np.ascontiguousarray(fresh, np.int32)
+        tokens = np.ascontiguousarray(tokens, np.int32)
+        if fresh.sum() != tokens.size:
+            raise ValueError(f"{tokens.size} tokens for {fresh.sum()} new positions")
+        n = int(tokens.size if every else (fresh > 0).sum())
+        out = {"entropy": np.zeros(n, np.float32), "top_id": np.zeros((n, top), np.int32), "top_logprob": np.zeros((n, top), np.float32)}
+        if given is not None:
+            given = np.ascontiguousarray(given, np.int32)
+            if given.size != n:
+                raise ValueError(f"{given.size} given tokens for {n} rows")
+            out["logprob"] = np.zeros(n, np.float32)
+        if logits:
+            out["logits"] = np.zeros((n, self.cfg["vocab_size"]), np.float32)
+        b = ModelBatch(int(fresh.size), int(every), top, ptr(fresh), ptr(tokens), ptr(given), ptr(out.get("logprob")), ptr(out["entropy"]),
+                       ptr(out["top_id"]), ptr(out["top_logprob"]), ptr(out.get("logits")))
+        check(self.lib.gmoe_model_step(self.h, C.byref(b), stream), "gmoe_model_step")
+        return out
+
+    def release(self, request, stream=None):
+        check(self.lib.gmoe_model_release(self.h, request, stream), "gmoe_model_release")
+
+    def free_pages(self):
+        return int(self.lib.gmoe_model_free_pages(self.h))
 
     def close(self):
         if self.h:
