@@ -197,8 +197,7 @@ __device__ static inline KaItem ka_uniform(KaItem m) {
 
 typedef _Float16 ka_h2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned u32x3 __attribute__((ext_vector_type(3)));
-typedef u32x3 u32x3_any __attribute__((aligned(1)));
+typedef unsigned u32_any __attribute__((aligned(1)));
 
 // Eight codes and their scale to eight halves.
 __device__ static inline a16_h8 ka_halves(unsigned codes, float scale) {
@@ -211,7 +210,7 @@ __device__ static inline a16_h8 ka_halves(unsigned codes, float scale) {
 struct KaRaw {
     u32x4 q0, q1;  // blocks j and 4 + j of the half (j = lane / 16)
     unsigned q2;   // the lane's eighth of block 8
-    u32x3 w;       // twelve scale bytes, the half's among them
+    unsigned w[3]; // twelve scale bytes, the half's among them
     unsigned on;   // all ones, or 0 where there is no such position
 };
 
@@ -282,7 +281,9 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
             x.q0 = *gbl((const u32x4 *)(row + at0));
             x.q1 = *gbl((const u32x4 *)(row + at1));
             x.q2 = *gbl((const unsigned *)(row + at2));
-            x.w = *(const GM_GLOBAL u32x3_any *)(row + ats);
+            // (word by word: a vector of three may be loaded as four, past the end of the pool's last row)
+#pragma unroll
+            for (int k = 0; k < 3; k++) x.w[k] = ((const GM_GLOBAL u32_any *)(row + ats))[k];
         };
         // the first pages, then the queries, then the first codes, so that they are under way together
         int page0 = -1, page = -1;
