@@ -123,8 +123,11 @@ __global__ __launch_bounds__(KV4_BLOCK) void k_kv4_read(Kv4Cache c, int n, const
         kv4_values(((const unsigned *)row)[i], row[16 * c.blocks + (i >> 2)], v);
     }
     if (VEC && have == 8) {
-        *(float4 *)dst = *(const float4 *)&v[0];
-        *(float4 *)(dst + 4) = *(const float4 *)&v[4];
+        // non-temporal: the values are a stream nobody reads back here, and the rows stay in the caches
+        // (8191 rows of 512 + 64: 6.3 us, 8.9 with plain stores; the next append 7.0, 7.7 after those)
+        typedef float f4 __attribute__((ext_vector_type(4)));
+        __builtin_nontemporal_store(*(const f4 *)&v[0], (f4 *)dst);
+        __builtin_nontemporal_store(*(const f4 *)&v[4], (f4 *)(dst + 4));
     } else {
 #pragma unroll
         for (int k = 0; k < 8; k++)
