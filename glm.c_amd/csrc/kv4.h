@@ -27,7 +27,8 @@ __host__ __device__ static inline int kv4_blocks(int kv, int rope) { return kv /
 //
 // Four lanes a block of 32 columns, eight columns a lane, a row's lanes side by side: a lane's
 // eight values are two 16-byte loads where the rows are aligned to that (VEC), its eight codes
-// one 4-byte store. Bound by the memory traffic, most of it the fp32 values.
+// one 4-byte store. Bound by the memory traffic, most of it the fp32 values: 8191 rows of 512 + 64 take 7.0 us
+// to write (21.5 MB, 3.1 TB/s) and 6.3 to read back (3.4 TB/s), 64 rows 3.4 and 3.1 (a launch).
 
 // The code of |v| = mag steps (mag >= 0): halves up to 2, ones up to 4, then twos, each rounded
 // to the even one at a tie (rint), at most 6.

@@ -4,11 +4,11 @@
 // or 3) and a unit a tile against KA_P positions. All units of a launch lie on one axis, tile after
 // tile, each tile led by KA_LEAD for what it costs to begin one; the axis is cut into one equal
 // share a block, so that every block has the same work whatever the lengths. A tile inside one
-// share is written where it belongs; one that the cuts part leaves a partial result a block, which k_kv4_merge joins. A
-// block has at most two partial results, of its first tile and its last. The lengths are device data,
-// so every block works out the axis by itself; a tile's place on it is a formula (ka_place),
-// near its units' number, and the units in a share follow from the place alone (ka_cut), so that
-// neighbours agree.
+// share is written where it belongs; one that the cuts part leaves a partial result a block, which
+// k_kv4_merge joins. A block has at most two partial results, of its first tile and its last. The
+// lengths are device data, so every block works out the axis by itself; a tile's place on it is a
+// formula (ka_place), near its units' number, and the units in a share follow from the place alone
+// (ka_cut), so that neighbours agree.
 //
 // Products. Both run on v_mfma_f32_16x16x32_f16. The cache's values are exact in fp16 (e2m1 times a
 // power of two that the format holds to fp16's range), so only the queries and the exponentials
@@ -28,6 +28,13 @@
 // The softmax of a tile and the scores of the next share a phase, in opposite order on the two waves of
 // a SIMD, so that the one's vector instructions run beside the other's matrix instructions; two barriers
 // a tile. Codes are requested a tile ahead, their pages two.
+//
+// Measured, 20 heads, ranks 512 + 64 (kernel + join): one token at 4096 positions 15.6 + 5.0 us, 64 requests
+// of 8 to 8192 positions 31.8 + 6.9 (36.7 MB of rows, 1.2 TB/s), 1023 tokens at 2977 before 387 + 12 (155
+// GFLOP, twice that with the split: 0.8 PFLOP/s of matrix instructions). What bounds it: a unit of three
+// operand tiles takes some 5400 clocks of a CU, of which its matrix instructions are 1630 of a SIMD's, its
+// vector instructions 2050 and shared memory 1800; two waves a SIMD (the registers hold no more) and two barriers a unit
+// overlap a third of that. Few rows: the beginning (lengths, table, codes: three waits on memory) and the join.
 //
 // Softmax reference: exponentials are taken against a row's reference, which follows the running
 // maximum only when a score passes it by 2^KA_SLACK, so that sums are rescaled a few times a

@@ -93,7 +93,7 @@ extern "C" int gmoe_page_maps(int device, const gmoe_batch *b, void *stream) {
     if (int rc = check_batch("gmoe_page_maps", b)) return rc;
     OnDevice on(device);
     if (on.err != hipSuccess) return failed("gmoe_page_maps: the device", on.err);
-    const unsigned grid = (unsigned)((b->max_tokens + PM_TOKENS - 1) / PM_TOKENS);
+    const unsigned grid = (unsigned)((b->max_tokens + PM_BLOCK - 1) / PM_BLOCK);
     hipLaunchKernelGGL(k_page_maps, dim3(grid), dim3(PM_BLOCK), 0, (hipStream_t)stream, *b, page_shift(b->page_size));
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? GMOE_OK : failed("gmoe_page_maps", e);
