@@ -30,7 +30,7 @@
 // a tile. Codes are requested a tile ahead, their pages two.
 //
 // Measured, 20 heads, ranks 512 + 64 (kernel + join): one token at 4096 positions 15.6 + 5.0 us, 64 requests
-// of 8 to 8192 positions 31.8 + 6.9 (36.7 MB of rows, 1.2 TB/s), 1023 tokens at 2977 before 387 + 12 (155
+// of 8 to 8192 positions 31.8 + 6.9 (36.7 MB of rows, 1.2 TB/s), 1023 tokens after 2977 389 + 12 (155
 // GFLOP, twice that with the split: 0.8 PFLOP/s of matrix instructions). What bounds it: a unit of three
 // operand tiles takes some 5400 clocks of a CU, of which its matrix instructions are 1630 of a SIMD's, its
 // vector instructions 2050 and shared memory 1800; two waves a SIMD (the registers hold no more) and two barriers a unit

@@ -8,7 +8,7 @@
 // j * page_size, which is one of its new tokens exactly where j is a new page.
 //
 // Latency bound at every size (a call moves 0.1 MB for 1000 requests): a wait on the lengths, two sums, a
-// search, a wait on the page. 1000 requests with some 9000 tokens: 6.7 us a call, as one request's (a launch
+// search, a wait on the page. 1000 requests with 7411 tokens: 6.7 us a call, as one request's (a launch
 // from the host alone is about that), with a token a thread and the first lengths in registers; 9.7
 // with four tokens a thread and lengths reread.
 #pragma once
