@@ -1201,6 +1201,7 @@ extern "C" int gmoe_model_open_pages(gmoe_model *m, int max_requests, int page_s
     m->rows_max = (int)std::min<size_t>(kStepRows, B);
     for (int n = 1; n <= m->rows_max; n++) m->score_bytes = std::max(m->score_bytes, gmoe_logprobs_workspace(n, c.vocab_size, GMOE_TOP_MAX));
     m->attend_bytes = gmoe_kv4_attend_workspace(c.n_heads, c.kv_lora_rank);
+    const size_t held = m->allocs.size();
     int rc = GMOE_OK;
     rc |= mdalloc(m, &m->pages, (size_t)c.attn_layers * n_pages * page_size * row);
     rc |= mdalloc(m, &m->table, R * width);
@@ -1214,7 +1215,11 @@ extern "C" int gmoe_model_open_pages(gmoe_model *m, int max_requests, int page_s
     rc |= mdalloc(m, &m->rows_out, (size_t)m->rows_max * (2 + 2 * GMOE_TOP_MAX));
     rc |= mdalloc(m, &m->attend_work, m->attend_bytes);
     rc |= mdalloc(m, &m->score_work, m->score_bytes);
-    if (rc) return GMOE_ERR_NOMEM;  // (what was allocated goes with the model)
+    if (rc) {  // as before the call, so that a smaller pool may follow
+        for (; m->allocs.size() > held; m->allocs.pop_back()) (void)hipFree(m->allocs.back());
+        (void)hipGetLastError();
+        return GMOE_ERR_NOMEM;
+    }
     std::vector<int32_t> ids((size_t)n_pages);
     for (int i = 0; i < n_pages; i++) ids[i] = n_pages - 1 - i;  // taken from the end: page 0 first
     MH_OK(hipMemcpy(m->free_pages, ids.data(), ids.size() * sizeof(int32_t), hipMemcpyHostToDevice));

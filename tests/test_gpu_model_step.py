@@ -237,6 +237,29 @@ def test_refused_steps_change_nothing():
 
 
 @pytest.mark.gpu
+def test_a_pool_that_does_not_fit_leaves_the_model_as_it_was():
+    cfg = dict(CFG, max_batch=1)
+    g, attn = gmoe.synth_model_weights(cfg, 2)
+    model = gmoe.Model(cfg)
+    try:
+        model.upload(g)
+        for l, a in enumerate(attn):
+            model.upload_attn(l, a)
+        want = model.forward_token(5, 0).copy()
+        with pytest.raises(RuntimeError, match=r"gmoe_model_open_pages failed \(-3\)"):
+            model.open_pages(4, 1 << 16, (1 << 15) - 1)  # 2^31 positions of 64 bytes in three layers: 412 GB
+        assert model.free_pages() == -1
+        assert np.array_equal(model.forward_token(5, 0), want)
+        with pytest.raises(RuntimeError, match=r"gmoe_model_step failed \(-1\)"):
+            model.step([1], [5])
+        model.open_pages(4, 16, 8)
+        model.step([1], [5])
+        assert model.free_pages() == 7
+    finally:
+        model.close()
+
+
+@pytest.mark.gpu
 def test_the_fp32_cache_is_left_alone():
     """A sequence decoded on the model's own cache gives the same bits with steps between its tokens."""
     g, attn, moe, steps, *_ = expected("mixed", SEEDS["mixed"])
