@@ -29,8 +29,8 @@
 // a SIMD, so that the one's vector instructions run beside the other's matrix instructions; two barriers
 // a tile. Codes are requested a tile ahead, their pages two.
 //
-// Measured, 20 heads, ranks 512 + 64 (kernel + join): one token at 4096 positions 15.6 + 5.0 us, 64 requests
-// of 8 to 8192 positions 31.8 + 6.9 (36.7 MB of rows, 1.2 TB/s), 1023 tokens after 2977 389 + 12 (155
+// Measured, 20 heads, ranks 512 + 64 (kernel + join): one token at 4096 positions 14.2 + 5.1 us, 64 requests
+// of 8 to 8192 positions 31.9 + 6.3 (36.7 MB of rows, 1.2 TB/s), 1023 tokens after 2977 389 + 12 (155
 // GFLOP, twice that with the split: 0.8 PFLOP/s of matrix instructions). What bounds it: a unit of three
 // operand tiles takes some 5400 clocks of a CU, of which its matrix instructions are 1630 of a SIMD's, its
 // vector instructions 2050 and shared memory 1800; two waves a SIMD (the registers hold no more) and two barriers a unit
@@ -41,6 +41,8 @@
 // chunk. They are scaled by 2^KA_UP for the split, whose error is then 2^-33 of the largest.
 #pragma once
 
+#include <algorithm>
+
 #include "kv4.h"
 #include "split16.h"
 
@@ -50,7 +52,6 @@
 #define KA_ROWS 24    // rows of the largest tile
 #define KA_HALF 9     // column blocks of a wave's half
 #define KA_GRID 256   // blocks: one a CU
-#define KA_SHARE 2    // least share of a block: with 1 a token at 4096 takes 14.2 + 6.4 us (the join), with 2 15.6 + 5.0
 #define KA_LEAD 4     // of a tile's beginning, in units (64 ragged requests: 39 us with 2, 32 with 4, 34 with 7)
 #define KA_SLACK 6.0f
 #define KA_UP 8
@@ -67,6 +68,7 @@ struct KaCut {
     int first, next; // slots of its partial results: first, next, next + 2, next + 4, ...
     int t0, row0, nr;
 };
+static_assert(sizeof(KaCut) == 6 * sizeof(int), "read as six words");
 
 struct Kv4Attn {
     Kv4Cache c;
@@ -152,7 +154,7 @@ __device__ static inline KaPlan ka_plan(const Kv4Attn &a, int rows, KaShared &sh
     }
     p.at = before + s - p.size;
     p.total = (uint64_t)readlane_d(total, 0);
-    p.share = max((uint64_t)KA_SHARE, (p.total + KA_GRID - 1) / KA_GRID);
+    p.share = max((uint64_t)1, (p.total + KA_GRID - 1) / KA_GRID);  // (2 at least: a token at 4096 15.6 us, with 1 14.2)
     return p;
 }
 
@@ -573,23 +575,50 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
 }
 
 // The cut tiles' partial results joined: out = sum_c w_c part_c / sum_c w_c l_c with w_c = 2^(ref_c - max
-// ref). A block has two rows of the tile that ends in share blockIdx.y; a row's threads have four columns
-// each and every other part.
+// ref). A block has two rows of the blockIdx.y-th cut tile and one of QUARTERS parts of their columns; a
+// row's threads have four columns each and every 2 QUARTERS-th part. Few tiles (one long sequence) are
+// joined by four times the blocks.
 #define KM_ROWS 2
-#define KM_GROUPS 2
-#define KM_COLS (KA_BLOCK / KM_ROWS / KM_GROUPS)
-static_assert(4 * KM_COLS >= 512, "a group's threads cover a row");
+#define KM_FEW 8  // tiles (joining a token's 64 parts: 5.1 us with quarters, 6.4 without; 64 tiles: 10.6 and 6.3)
+#define KM_THREADS (KA_BLOCK / KM_ROWS)
+template <int QUARTERS>
 __global__ __launch_bounds__(KA_BLOCK) void k_kv4_merge(Kv4Attn a) {
+    constexpr int COLS = 128 / QUARTERS, GROUPS = KM_THREADS / COLS;  // threads of a row's part, groups of them
+    static_assert(4 * 128 >= 512 && KM_THREADS % COLS == 0, "the parts cover a row");
+    __shared__ int cut[6];
+    __shared__ int found[KA_GRID / 64];
     __shared__ float wgt[KM_ROWS][KA_GRID];
-    __shared__ float red[KM_ROWS][KA_WAVES / KM_ROWS], red2[KM_ROWS][KA_WAVES / KM_ROWS];
-    __shared__ __align__(16) float4 sum[KM_ROWS][KM_COLS];
-    const KaCut m = a.cuts[blockIdx.y];
-    const int kv = a.c.kv, tid = threadIdx.x;
-    const int sub = __builtin_amdgcn_readfirstlane(tid / (KA_BLOCK / KM_ROWS)), t = tid % (KA_BLOCK / KM_ROWS), rr = blockIdx.x * KM_ROWS + sub;
-    if (m.k == 0 || (int)blockIdx.x * KM_ROWS >= m.nr) return;
+    __shared__ float red[KM_ROWS][4], red2[KM_ROWS][4];
+    __shared__ __align__(16) float4 sum[KM_ROWS][GROUPS - 1][COLS];
+    const int kv = a.c.kv, tid = threadIdx.x, pair = blockIdx.x / QUARTERS;
+    // the blockIdx.y-th of the shares that a cut tile ends in
+    const bool has = tid < KA_GRID;
+    // (word by word: as a struct of each thread's the compiler keeps it in shared memory, and reads the launch's
+    // packet for its place there: 14 us)
+    const int *share = (const int *)(a.cuts + (has ? tid : 0));
+    int f[6];
+#pragma unroll
+    for (int i = 0; i < 6; i++) f[i] = share[i];
+    const unsigned long long ends = __ballot(has && f[0] > 0);
+    if (has && (tid & 63) == 0) found[tid >> 6] = __popcll(ends);
+    __syncthreads();
+    int rank = __popcll(ends & ((1ull << (tid & 63)) - 1)), all = 0;
+#pragma unroll
+    for (int i = 0; i < KA_GRID / 64; i++) {
+        if (i < tid >> 6) rank += found[i];
+        all += found[i];
+    }
+    if ((int)blockIdx.y >= all) return;
+    if (has && f[0] > 0 && rank == (int)blockIdx.y)
+#pragma unroll
+        for (int i = 0; i < 6; i++) cut[i] = f[i];
+    __syncthreads();
+    const KaCut m = {cut[0], cut[1], cut[2], cut[3], cut[4], cut[5]};
+    if (pair * KM_ROWS >= m.nr) return;
+    const int sub = __builtin_amdgcn_readfirstlane(tid / KM_THREADS), t = tid % KM_THREADS, rr = pair * KM_ROWS + sub;
     const bool there = rr < m.nr;
     auto at = [&](int c) { return (size_t)(c == 0 ? m.first : m.next + 2 * (c - 1)) * KA_ROWS + rr; };
-    static_assert(KA_GRID <= KA_BLOCK / KM_ROWS, "a thread a part");
+    static_assert(KA_GRID <= KM_THREADS, "a thread a part");
     float pm = -INFINITY, pl = 0.0f;
     if (there && t < m.k) {
         pm = a.part_ml[at(t) * 2];
@@ -606,11 +635,11 @@ __global__ __launch_bounds__(KA_BLOCK) void k_kv4_merge(Kv4Attn a) {
     if ((t & 63) == 0) red2[sub][t >> 6] = l;
     __syncthreads();
     l = (red2[sub][0] + red2[sub][1]) + (red2[sub][2] + red2[sub][3]);
-    const int grp = t / KM_COLS, col = 4 * (t % KM_COLS);
+    const int grp = t / COLS, col = 4 * (t % COLS + COLS * (blockIdx.x % QUARTERS));
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (there && col < kv) {
 #pragma unroll 8
-        for (int c = grp; c < m.k; c += KM_GROUPS) {
+        for (int c = grp; c < m.k; c += GROUPS) {
             const float4 v = *(const float4 *)(a.part + at(c) * kv + col);
             const float x = wgt[sub][c];
             s.x = fmaf(x, v.x, s.x);
@@ -619,20 +648,32 @@ __global__ __launch_bounds__(KA_BLOCK) void k_kv4_merge(Kv4Attn a) {
             s.w = fmaf(x, v.w, s.w);
         }
     }
-    if (grp == 1) sum[sub][t % KM_COLS] = s;
+    if (grp > 0) sum[sub][grp - 1][t % COLS] = s;
     __syncthreads();
     if (there && col < kv && grp == 0) {
-        const float4 v = sum[sub][t];
+#pragma unroll
+        for (int i = 0; i + 1 < GROUPS; i++) {
+            const float4 v = sum[sub][i][t % COLS];
+            s.x += v.x;
+            s.y += v.y;
+            s.z += v.z;
+            s.w += v.w;
+        }
         const int g = m.row0 + rr, tok = g / a.H;
         float *dst = a.out + (m.t0 + tok) * a.ld_out + (int64_t)(g - tok * a.H) * kv + col;
         const float f = l == 0.0f ? 0.0f : 1.0f / l;
-        dst[0] = (s.x + v.x) * f;
-        dst[1] = (s.y + v.y) * f;
-        dst[2] = (s.z + v.z) * f;
-        dst[3] = (s.w + v.w) * f;
+        dst[0] = s.x * f;
+        dst[1] = s.y * f;
+        dst[2] = s.z * f;
+        dst[3] = s.w * f;
     }
 }
-static_assert(KM_GROUPS == 2 && KA_WAVES / KM_ROWS == 4, "two groups, four waves a row");
+static_assert(KM_THREADS == 256, "four waves a row");
+
+// The most tiles a launch can cut, of those that a step of up to `tokens` tokens of R requests has.
+static inline int ka_cut_tiles(long long tokens, int R, int H, int mt) {
+    return (int)std::min<long long>(KA_GRID, tokens * H / (8 * mt) + R);
+}
 
 // Operand tiles a row tile for rows of a request's step, by the cost of the tiles it takes: each
 // converts the cache's codes once (about one operand tile's products) and multiplies MT operand tiles.

@@ -190,7 +190,9 @@ extern "C" int gmoe_kv4_attend(int device, const gmoe_kv4 *c, const gmoe_batch *
     if (mt == 1) hipLaunchKernelGGL(k_kv4_attend<1>, dim3(KA_GRID), dim3(KA_BLOCK), 0, st, a);
     else if (mt == 2) hipLaunchKernelGGL(k_kv4_attend<2>, dim3(KA_GRID), dim3(KA_BLOCK), 0, st, a);
     else hipLaunchKernelGGL(k_kv4_attend<3>, dim3(KA_GRID), dim3(KA_BLOCK), 0, st, a);
-    hipLaunchKernelGGL(k_kv4_merge, dim3(8 * mt / KM_ROWS, KA_GRID), dim3(KA_BLOCK), 0, st, a);
+    const unsigned tiles = (unsigned)ka_cut_tiles(b->max_tokens, a.R, a.H, mt), pairs = 8 * mt / KM_ROWS;
+    if (tiles <= KM_FEW) hipLaunchKernelGGL(k_kv4_merge<4>, dim3(4 * pairs, tiles), dim3(KA_BLOCK), 0, st, a);
+    else hipLaunchKernelGGL(k_kv4_merge<1>, dim3(pairs, tiles), dim3(KA_BLOCK), 0, st, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? GMOE_OK : failed("gmoe_kv4_attend", e);
 }

@@ -117,8 +117,8 @@ typedef struct gmoe_kv4_heads {
 /* The attention of the step's tokens over their requests' cached positions (infer.c:1017-1058
  * on the paged form): for token t at position p of its request and head h, over positions
  * 0 .. p, out = sum_j softmax_j(scale (q_abs . comp_j + q_pe . pe_j)) comp_j. Reads of b the
- * sizes, table, offsets and context (as gmoe_page_maps leaves them; the step's own rows are
- * appended first). A position whose page is outside the pool is not attended; a token that
+ * sizes, table, offsets (at most max_tokens, rising) and context, as gmoe_page_maps leaves them; the
+ * step's own rows are appended first. A position whose page is outside the pool is not attended; a token that
  * attends none (a short request's) gets zeros. Tokens past offsets[R] are not written. fp32
  * in and out; scores, exponentials and sums in fp32. */
 int gmoe_kv4_attend(int device, const gmoe_kv4 *c, const gmoe_batch *b, const gmoe_kv4_heads *h, void *stream);
