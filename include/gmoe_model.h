@@ -119,21 +119,23 @@ int gmoe_model_prefill(gmoe_model *m, const int32_t *tokens, int n, int pos0, fl
 int gmoe_model_read_cache(gmoe_model *m, int layer, int pos0, int n, float *comp_out, float *pe_out, void *stream);
 
 /* ---- several requests at once ---------------------------------------------------------------
- * A model serves up to max_requests requests, numbered from 0, over a paged latent cache in
- * 4 bits (gmoe_serve.h) beside its own fp32 cache, which these calls leave alone: a step
- * takes new tokens of any of them, whole prompts or parts of one and single tokens side by
- * side. Its products, MoE layers and LM head run once for all the step's tokens; the page tables
- * come from gmoe_page_maps, each layer's cache from gmoe_kv4_append and gmoe_kv4_attend, what is
- * returned from gmoe_logprobs. The cache in 4 bits is a 7.2th of the fp32 one and changes the
- * results: its entries are rounded to 8 magnitudes a sign and a power of two a 32 columns. */
+ * A model serves up to max_requests requests, numbered from 0, over a paged latent cache in 4
+ * bits (gmoe_serve.h) beside its own fp32 cache, which these calls leave alone: a step takes
+ * new tokens of any of them, whole prompts or parts of one and single tokens side by side.
+ * Its products, MoE layers and LM head run once for all the step's tokens; the page tables
+ * come from gmoe_page_maps, each layer's cache from gmoe_kv4_append and gmoe_kv4_attend, what
+ * is returned from gmoe_logprobs. At ranks 512 + 64 a position takes 320 bytes a layer instead
+ * of 2304, and results differ by the rounding: 8 magnitudes and a sign, a power of two a 32
+ * columns. */
 
 /* Reserves n_pages pages of page_size positions (a power of two) for every attention layer,
  * and what a step of up to the model's max_batch tokens needs. A request may have cache_cap
- * positions (the rope table's). Once a model. */
+ * positions (the rope table's). Once a model; after GMOE_ERR_NOMEM a smaller pool may follow. */
 int gmoe_model_open_pages(gmoe_model *m, int max_requests, int page_size, int n_pages);
 
-/* A step, in host memory. Its rows are what the LM head runs on: the last new token of each request
- * that has any, in the requests' order, or with `every` each new token. */
+/* A step, in host memory. Its rows are what the LM head runs on: the last new token of each
+ * request that has any, in the requests' order, or with `every` each new token. A token id
+ * outside the vocabulary counts as 0 (infer.c:1781); a given one has NaN. */
 typedef struct gmoe_model_batch {
     int32_t n_requests;        /* requests 0 .. n_requests - 1 take part */
     int32_t every;
@@ -148,8 +150,9 @@ typedef struct gmoe_model_batch {
     float *logits;             /* [rows][vocab_size], or NULL */
 } gmoe_model_batch;
 
-/* One step on `stream`, then a synchronisation. The requests' positions go on from where the last step
- * left them. GMOE_ERR_NOMEM, with nothing changed, when the pages left do not hold the step. */
+/* One step on `stream`, then a synchronisation. The requests' positions go on from where the
+ * last step left them; after an error they stay there. GMOE_ERR_NOMEM when the pages left do
+ * not hold the step. */
 int gmoe_model_step(gmoe_model *m, const gmoe_model_batch *b, void *stream);
 
 /* Ends a request: its pages are free and it may begin anew at position 0. Synchronises `stream`. */

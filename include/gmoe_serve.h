@@ -10,9 +10,9 @@
  * Every pointer is device memory of the caller's on GPU `device`, the current device or
  * not; a call leaves the current device as it was. Nothing is allocated and nothing is kept
  * from one call for the next: a call is enqueued on `stream` (a hipStream_t as void*, NULL =
- * default stream of `device`) and may be captured into a graph. Arguments that the host can see are checked
- * before anything is enqueued; lengths, slots, pages and token ids are device data, and what
- * a kernel does with those out of range is said at each. Return codes and gmoe_last_error()
+ * default stream of `device`) and may be captured into a graph. Arguments that the host can
+ * see are checked before anything is enqueued; lengths, slots, pages and token ids are device
+ * data, and what a kernel does with those out of range is said at each. Return codes and gmoe_last_error()
  * as in gmoe.h. Two calls may overlap when neither writes what the other reads or writes,
  * workspaces included.
  */

@@ -8,6 +8,10 @@ of two magnitudes that fp32 could round it the other way. So the 64-bit model is
 16 times the largest difference of the two (numpy's sums and the kernels' round in different orders, both
 by halves of 2^-23 an operation) must be less than the smallest distance from a middle, which picks the seeds
 here on the CPU, and bounds what the results may be off by."""
+import ctypes as C
+import os
+import subprocess
+
 import numpy as np
 import pytest
 
@@ -278,6 +282,17 @@ def test_the_fp32_cache_is_left_alone():
         ctx.close()
         plain.close()
         ctx_p.close()
+
+
+def test_ctypes_struct_matches_the_header(tmp_path):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "gmoe_model.h"', "int main(void) {",
+             'printf("%zu\\n", sizeof(gmoe_model_batch));']
+    lines += [f'printf("%zu\\n", offsetof(gmoe_model_batch, {f}));' for f, _ in gmoe.ModelBatch._fields_]
+    (tmp_path / "probe.c").write_text("\n".join(lines + ["return 0; }"]))
+    subprocess.run(["gcc", "-std=c11", "-o", str(tmp_path / "probe"), str(tmp_path / "probe.c"), f"-I{root}/include"], check=True)
+    out = subprocess.run([str(tmp_path / "probe")], check=True, capture_output=True, text=True).stdout.split()
+    assert [int(v) for v in out] == [C.sizeof(gmoe.ModelBatch)] + [getattr(gmoe.ModelBatch, f).offset for f, _ in gmoe.ModelBatch._fields_]
 
 
 def test_refusals_without_a_model():
