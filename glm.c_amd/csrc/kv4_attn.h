@@ -86,7 +86,8 @@ struct Kv4Attn {
 
 // ---- the split of a launch -------------------------------------------------------------------
 
-__device__ static inline unsigned ka_tiles(const Kv4Attn &a, int fresh, int rows) { return (unsigned)(fresh * a.H + rows - 1) / rows; }  // (fresh * H < 2^27)
+// (fresh * H < 2^27)
+__device__ static inline unsigned ka_tiles(const Kv4Attn &a, int fresh, int rows) { return (unsigned)(fresh * a.H + rows - 1) / rows; }
 
 // The place on the axis of tile i of a request whose first token has `first` positions before it: a
 // trapezoid's area, rounded, so that it needs no sum over the tiles. Rises by over KA_LEAD a tile.
@@ -415,7 +416,8 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
         // where the lane finds its position's scores and puts its pair of positions' first parts, or the second,
         // but for the row
         const int rat = lane * KA_SROW, rmix = (lane & 8) >> 1 ^ (lane & 16) >> 3;
-        const int pat = (32 * (lane >> 5) + 8 * ((lane & 15) >> 2) + 4 * ((lane & 31) >> 4) + (lane & 2)) ^ 16 * (lane & 1), podd = 2 * KA_PROW * (lane & 1);
+        const int pat = (32 * (lane >> 5) + 8 * ((lane & 15) >> 2) + 4 * ((lane & 31) >> 4) + (lane & 2)) ^ 16 * (lane & 1);
+        const int podd = 2 * KA_PROW * (lane & 1);
         const unsigned pick = lane & 1 ? 0x03020706u : 0x05040100u;  // of (the partner's, the lane's) pair of parts
         auto softmax = [&](int j) {
             const int s = s0 + KA_P * j + lane;
@@ -462,7 +464,8 @@ __global__ __launch_bounds__(KA_BLOCK, 2) void k_kv4_attend(Kv4Attn a) {
                 ka_h2 both;
                 both.x = (_Float16)e;
                 both.y = (_Float16)fmaf((float)both.x, -1.0f, e);
-                const unsigned me = __builtin_bit_cast(unsigned, both), other = (unsigned)__builtin_amdgcn_update_dpp(0, (int)me, DPP_QUAD_1032, 0xF, 0xF, false);
+                const unsigned me = __builtin_bit_cast(unsigned, both);
+                const unsigned other = (unsigned)__builtin_amdgcn_update_dpp(0, (int)me, DPP_QUAD_1032, 0xF, 0xF, false);
                 const int r = RPW * w + i, o = 16 * (r >> 3) + 4 * ((r & 7) >> 1) + (r & 1);  // (the second part's row is o + 2)
                 *(unsigned *)&pr[o * KA_PROW + podd + (pat ^ 8 * ((o & 7) ^ (o >> 3 & 1)))] = __builtin_amdgcn_perm(other, me, pick);
             }
